@@ -269,11 +269,11 @@ def _plain_reserve(st, b):
     dev = b.buf.device
     ids, add = st["list"].long(), st["add"].long()
     at = torch.arange(ids.numel(), device=dev)
-    ok = (ids >= 0) & (ids < n_seqs) & (add >= 0)
-    s = torch.where(ok, ids, 0)
+    named = (ids >= 0) & (ids < n_seqs)
+    s = torch.where(named, ids, 0)
     tokens = b.lengths[s].long()
     old, new = _held(tokens, rows), _held(tokens + add, rows)
-    ok = ok & _first(s, ok, n_seqs) & (new <= width)
+    ok = named & _first(s, named, n_seqs) & (add >= 0) & (new <= width)
     # a last page with room, held by others too
     partial = ok & (add > 0) & (tokens % rows != 0)
     tail = torch.where(partial, b.tables[s, (old - 1).clamp(min=0)].long(), n_pages)
@@ -309,10 +309,11 @@ def _plain_reserve(st, b):
 def _plain_fork(st, b):
     rows, n_seqs = st["rows"], st["seqs"]
     parents, children = st["list"].long(), st["children"].long()
-    ok = (parents >= 0) & (parents < n_seqs) & (children >= 0) & (children < n_seqs)
-    p, c = torch.where(ok, parents, 0), torch.where(ok, children, 0)
-    named = torch.zeros(n_seqs + 1, dtype=torch.bool, device=p.device).index_fill_(0, torch.where((children >= 0) & (children < n_seqs), children, n_seqs), True)
-    ok = ok & _first(c, ok, n_seqs) & ~named[p] & (b.lengths[c] == 0)
+    some = (children >= 0) & (children < n_seqs)
+    ok = some & (parents >= 0) & (parents < n_seqs)
+    p, c = torch.where(ok, parents, 0), torch.where(some, children, 0)
+    named = torch.zeros(n_seqs + 1, dtype=torch.bool, device=p.device).index_fill_(0, torch.where(some, children, n_seqs), True)
+    ok = ok & _first(c, some, n_seqs) & ~named[p] & (b.lengths[c] == 0)
     st["granted"].copy_(ok)
     p, c = p[ok], c[ok]
     tokens = b.lengths[p]
@@ -443,9 +444,9 @@ def exact(case, seed):
     if case["op"] == "reserve":
         free, taken = np.nonzero(refs == 0)[0], 0
         for i, (s, a) in enumerate(zip(ids, st["add"].tolist())):
-            if not 0 <= s < case["seqs"] or a < 0 or s in named or -(-(lengths[s] + a) // rows) > width:
+            again, named = s in named, named | {s}
+            if not 0 <= s < case["seqs"] or again or a < 0 or -(-(lengths[s] + a) // rows) > width:
                 continue
-            named.add(s)
             o, m = -(-lengths[s] // rows), -(-(lengths[s] + a) // rows)
             apart = a > 0 and lengths[s] % rows != 0 and refs[tables[s, o - 1]] > 1
             if m - o + apart > len(free) - taken:
@@ -461,9 +462,9 @@ def exact(case, seed):
     elif case["op"] == "fork":
         children = st["children"].tolist()
         for i, (p, c) in enumerate(zip(ids, children)):
-            if not (0 <= p < case["seqs"] and 0 <= c < case["seqs"]) or c in named or p in children or lengths[c]:
+            again, named = c in named, named | {c}
+            if not (0 <= p < case["seqs"] and 0 <= c < case["seqs"]) or again or p in children or lengths[c]:
                 continue
-            named.add(c)
             held = tables[p, :-(-lengths[p] // rows)]
             tables[c, :len(held)] = held
             refs[held] += 1
