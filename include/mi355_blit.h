@@ -341,6 +341,160 @@ int mi355_blit_plan_rect_route(const mi355_pitched_ptr_t* dst, const mi355_dim3_
                                const mi355_dim3_t* range, const mi355_blit_tuning_t* tuning, uint32_t route,
                                mi355_blit_rect_plan_t* out);
 
+/* ---------------------------------------------------------------------------
+ * Pages of a key/value cache.
+ *
+ * A language model that serves many sequences keeps their keys and values in
+ * pages of a few tokens each, so that memory is handed out a page at a time and
+ * sequences can share what they have in common.  These calls are the memory
+ * side of that: they copy pages, hand them out, share them, take them back and
+ * move them together.  No counterpart in the reference.
+ *
+ * A pool has planes (one for the keys and one for the values of every layer;
+ * scales of a quantised cache are planes of their own).  Page q of a plane is at
+ * base + q * pitch and is `runs` runs of `rows` rows of row_bytes bytes, one
+ * behind the other: one run for the layout [token][head][dim], one run for each
+ * head for [head][token][dim].  What the bytes mean does not matter, and any
+ * address, pitch and row length will do (multiples of 16 are fastest).
+ *
+ * A book says which sequence holds which pages.  It is one buffer of 32-bit
+ * words in the GPU's memory that the caller allocates (mi355_blit_pages_book has
+ * its size and the places of its parts), so that attention kernels read it in
+ * place, and a copy of the buffer is a copy of the whole state:
+ *   head        word 0: the moves of the last compaction; the others are 0
+ *   lengths     [max_seqs] tokens of each sequence, 0 for an empty one
+ *   ref_counts  [num_pages] how many sequences hold a page
+ *   free_bits   bit q % 32 of word q / 32 is 1 where ref_counts[q] is 0
+ *   tables      [max_seqs][max_pages_per_seq]; sequence s holds the pages
+ *               tables[s][0 .. ceil(lengths[s] / rows)); entries from there on
+ *               mean nothing and are left as they are
+ * The calls keep these in line with one another.  A caller that changes the
+ * buffer itself keeps them in line too; where it does not, what the calls make
+ * of the book is wrong, but nothing outside the pool and the book is touched:
+ * numbers of pages and sequences are checked on the device.
+ *
+ * Everything a call reads or writes is in the GPU's memory (lists of sequences
+ * and of pages, counts, what was granted), nothing is read back, and nothing is
+ * allocated: a call is one to four kernel launches and may be recorded into a HIP graph.
+ * Lists are arrays of int32_t; a number that is out of range (-1, say) is an
+ * entry to pass over.  They are read when the commands run and have to stay as
+ * they are until then.  Calls on one pool use its book and its work memory: those that may overlap --
+ * on different streams, or in graphs that are replayed at the same time, without an
+ * ordering between them -- race and are the caller's to order, except
+ * copies from and to pages that nothing else in flight writes.  stream is a
+ * hipStream_t, or NULL for the handle's own.  Like the allocation-free batch
+ * these commands are not entered in the pending-bytes ledger. */
+typedef struct mi355_blit_pages mi355_blit_pages_t;
+
+/* Sequences that one call can name, sequences and pages that a book can have. */
+#define MI355_BLIT_PAGES_MAX_LIST 8192
+#define MI355_BLIT_PAGES_MAX_SEQS 65536
+#define MI355_BLIT_PAGES_MAX_PAGES 4194240
+
+typedef struct {
+  void* base;         /* page 0 */
+  uint64_t pitch;     /* bytes from a page to the next, at least runs * rows * row_bytes */
+  uint32_t row_bytes; /* bytes of one token in one run */
+  uint32_t runs;
+} mi355_blit_plane_t;
+
+typedef struct {
+  const mi355_blit_plane_t* planes; /* host memory; read by mi355_blit_pages_create only */
+  uint32_t n_planes;
+  uint32_t num_pages;
+  uint32_t rows;              /* tokens of a page */
+  uint32_t max_seqs;          /* 0, with the next field 0 and book NULL: a pool */
+  uint32_t max_pages_per_seq; /* without a book, for copies only */
+  uint32_t pad;               /* 0 */
+  int32_t* book;              /* 16-byte aligned device memory, `words` words of
+                                 mi355_blit_pages_book; its contents are the
+                                 caller's (mi355_blit_pages_reset empties it) */
+} mi355_blit_pages_desc_t;
+
+/* Where the parts of a book start, and its size, in 32-bit words. */
+typedef struct {
+  uint64_t lengths, ref_counts, free_bits, tables, words;
+} mi355_blit_book_t;
+
+/* Pure host arithmetic.  A zero -> INVALID_ARGUMENT, more than the limits above
+ * -> OUT_OF_RESOURCES. */
+int mi355_blit_pages_book(uint32_t num_pages, uint32_t max_seqs, uint32_t max_pages_per_seq, mi355_blit_book_t* out);
+
+/* A pool, or a pool and its book, on the handle's GPU.  Allocates the work
+ * memory of the calls (12 bytes for each page, 32 for each 4 KiB of a page
+ * over all planes), so it cannot be called while a stream is being captured,
+ * and neither can mi355_blit_pages_destroy.  A missing plane or base, zero pages, rows,
+ * runs or row_bytes, a pitch below the page's bytes, a book without sequences
+ * or the other way round -> INVALID_ARGUMENT.  More than 4096 planes, a page of
+ * more than 2^31-1 bytes in one plane, sequences of more than 2^31-1 tokens,
+ * 2^32 pieces of 4 KiB or more in the pool, or more than the limits above -> OUT_OF_RESOURCES.
+ * The planes' and the book's memory stay the caller's and have to outlive the
+ * object, and the object has to be destroyed before the handle. */
+int mi355_blit_pages_create(mi355_blit_t* h, const mi355_blit_pages_desc_t* desc, mi355_blit_pages_t** out);
+
+/* Waits for the GPU, then frees the work memory.  Graphs that hold calls on the
+ * object cannot be replayed any more. */
+int mi355_blit_pages_destroy(mi355_blit_pages_t* p);
+
+/* Empties the book: no tokens, every page free, -1 in every table entry.
+ * INVALID_ARGUMENT without a book (and so for the calls below but the copy). */
+int mi355_blit_pages_reset(mi355_blit_pages_t* p, void* stream);
+
+/* Pages src_pages[i] of pool `src` to pages dst_pages[i] of pool `dst`, i < n,
+ * in all planes.  valid_rows[i] (NULL: all) is how many rows of every run are
+ * copied, the first ones; the rows behind them are left as they are.  The two
+ * may be one pool or two with the same rows and the same row_bytes and runs in
+ * each plane (bases and pitches may differ), on the same GPU; either may be host memory that the GPU can
+ * access, with the route that says so (MI355_BLIT_ROUTE_*, as in
+ * mi355_blit_copy_route).  A sequence's row of the tables is such a list.
+ * Lists that name a page as a destination twice, or both as a source and as a destination,
+ * leave the bytes of that page undefined, as overlapping copies do.  NULL
+ * list with n > 0, pools that differ -> INVALID_ARGUMENT; n pages of 2^32
+ * pieces of 4 KiB or more -> OUT_OF_RESOURCES; n == 0 -> SUCCESS without a launch.
+ * No book is read or written. */
+int mi355_blit_pages_copy(mi355_blit_pages_t* dst, const int32_t* dst_pages, mi355_blit_pages_t* src,
+                          const int32_t* src_pages, const int32_t* valid_rows, size_t n, uint32_t route,
+                          void* stream);
+
+/* Room for more[i] further tokens of sequence seqs[i]: lengths and tables are
+ * those with the tokens in place, whose rows the caller then writes.  Entries
+ * are served in order, each with the lowest pages that are free.  A sequence
+ * whose last page has room but is held by others too gets a page of its
+ * own for it: the rows that are in use are copied, in all planes, and the others'
+ * count goes down by one (the last to hold a page keeps it).  An entry
+ * is refused, and its sequence left as it is, if its number is out of range, an earlier
+ * entry names the sequence, more[i] is negative, or the table has no room for that many
+ * pages; the first entry for which not enough pages are free ends the call, and
+ * it and all behind it are refused.  granted[i] (may be NULL) is 1 for a served
+ * entry, 0 for a refused one.  NULL list with n > 0 -> INVALID_ARGUMENT, n >
+ * MI355_BLIT_PAGES_MAX_LIST -> OUT_OF_RESOURCES (so for the next two). */
+int mi355_blit_pages_reserve(mi355_blit_pages_t* p, const int32_t* seqs, const int32_t* more, size_t n,
+                             int32_t* granted, void* stream);
+
+/* Sequence children[i] becomes a second sequence of parents[i]'s tokens that
+ * holds the same pages; no page is copied until one of the two grows
+ * (mi355_blit_pages_reserve).  The parents are as they were before the call.
+ * Refused, and the child left as it is: numbers out of range, a child that has
+ * tokens, one that an earlier entry names too, one whose parent the call names as
+ * a child.  granted as above. */
+int mi355_blit_pages_fork(mi355_blit_pages_t* p, const int32_t* parents, const int32_t* children, size_t n,
+                          int32_t* granted, void* stream);
+
+/* Sequence seqs[i] keeps its first keep[i] tokens (keep NULL: none); pages it
+ * does not need for them lose a holder, and are free when they have none.
+ * keep[i] negative, or not below the sequence's length: nothing happens.  A
+ * sequence that is named twice keeps the fewer tokens of the two. */
+int mi355_blit_pages_free(mi355_blit_pages_t* p, const int32_t* seqs, const int32_t* keep, size_t n, void* stream);
+
+/* Moves the highest pages in use to the lowest free ones, as long as that moves
+ * them down, max_moves of them at most, so that the pages in use come to lie at the
+ * pool's start.  Rows, counts, free bits and tables follow; the bytes of a page
+ * that has moved away are left.  The number of moves is left in the book's
+ * head, and moves (NULL, or room for max_moves pairs) gets {from, to} of each,
+ * the highest page first, for a caller that knows pages by number.
+ * max_moves == 0 -> SUCCESS without a launch. */
+int mi355_blit_pages_compact(mi355_blit_pages_t* p, uint32_t max_moves, int32_t* moves, void* stream);
+
 /* Decrements an HSA signal by 1 from the GPU once every command submitted
  * before it on the stream has completed, and wakes its waiters: replaces the
  * completion_signal field of the reference's dispatch packet

@@ -19,6 +19,7 @@ ROCR_TEST = os.path.join(LIB_DIR, "test_rocr_blit")
 ORACLE_LIB = os.path.join(ORACLE_DIR, "libblit_oracle.so")
 HOST_LOGIC_TEST = os.path.join(LIB_DIR, "test_host_logic")
 KERNELS_ON_CPU_TEST = os.path.join(LIB_DIR, "test_kernels_on_cpu")
+PAGES_ON_CPU_TEST = os.path.join(LIB_DIR, "test_pages_on_cpu")
 XCD_PROGRESS = os.path.join(LIB_DIR, "xcd_progress")
 
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
@@ -119,18 +120,27 @@ def build_host_logic_test():
     return HOST_LOGIC_TEST
 
 
-def build_kernels_on_cpu_test():
-    """The blit kernels compiled for the host over tests/cpp/lane_emulation.h
-    (lanes in lock step, every access checked), under AddressSanitizer and
-    UBSan."""
-    test_src = os.path.join(ROOT, "tests", "cpp", "test_kernels_on_cpu.cpp")
+def _build_on_cpu_test(name, exe):
+    test_src = os.path.join(ROOT, "tests", "cpp", name)
     if not os.path.exists(test_src):
         return None
     os.makedirs(LIB_DIR, exist_ok=True)
     _run(["g++", "-O1", "-g", "-std=c++17", "-Wall", "-Wno-unknown-pragmas", "-fsanitize=address,undefined",
           "-fno-sanitize-recover=all", "-static-libasan", "-static-libubsan", "-I", INCLUDE, "-I", CSRC,
-          "-I", os.path.join(ROOT, "tests", "cpp"), "-o", KERNELS_ON_CPU_TEST, test_src])
-    return KERNELS_ON_CPU_TEST
+          "-I", os.path.join(ROOT, "tests", "cpp"), "-o", exe, test_src])
+    return exe
+
+
+def build_kernels_on_cpu_test():
+    """The blit kernels compiled for the host over tests/cpp/lane_emulation.h
+    (lanes in lock step, every access checked), under AddressSanitizer and
+    UBSan."""
+    return _build_on_cpu_test("test_kernels_on_cpu.cpp", KERNELS_ON_CPU_TEST)
+
+
+def build_pages_on_cpu_test():
+    """The page kernels, the same way."""
+    return _build_on_cpu_test("test_pages_on_cpu.cpp", PAGES_ON_CPU_TEST)
 
 
 def build_oracle():
@@ -157,7 +167,8 @@ def build_all():
     if r:
         out.append(r)
     out.append(build_oracle())
-    for t in (build_rocr_test(), build_host_logic_test(), build_kernels_on_cpu_test(), build_xcd_progress()):
+    for t in (build_rocr_test(), build_host_logic_test(), build_kernels_on_cpu_test(),
+              build_pages_on_cpu_test(), build_xcd_progress()):
         if t:
             out.append(t)
     return out

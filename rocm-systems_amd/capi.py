@@ -19,6 +19,9 @@ KERNEL_FILL = 2
 KERNEL_COPY_BATCH = 3
 KERNEL_COPY_RECT = 4
 NOALLOC_MAX_COPIES = 65536
+PAGES_MAX_LIST = 8192
+PAGES_MAX_SEQS = 65536
+PAGES_MAX_PAGES = 4194240
 ENGINE_NONE = 0
 ENGINE_BLIT_KERNEL = 1
 ENGINE_SDMA = 2
@@ -78,6 +81,22 @@ class RectPlan(C.Structure):
     ]
 
 
+class Plane(C.Structure):
+    _fields_ = [("base", C.c_void_p), ("pitch", C.c_uint64), ("row_bytes", C.c_uint32), ("runs", C.c_uint32)]
+
+
+class PagesDesc(C.Structure):
+    _fields_ = [
+        ("planes", C.POINTER(Plane)), ("n_planes", C.c_uint32), ("num_pages", C.c_uint32), ("rows", C.c_uint32),
+        ("max_seqs", C.c_uint32), ("max_pages_per_seq", C.c_uint32), ("pad", C.c_uint32), ("book", C.c_void_p),
+    ]
+
+
+class Book(C.Structure):
+    """Where the parts of a book start, and its size, in 32-bit words."""
+    _fields_ = [(n, C.c_uint64) for n in ("lengths", "ref_counts", "free_bits", "tables", "words")]
+
+
 def rect_args(dst, dst_offset, src, src_offset, extent):
     """(base, pitch, slice) and (x, y, z) tuples -> ctypes structures; None stays None."""
     def ptr(t):
@@ -107,6 +126,16 @@ SIGNATURES = {
     "mi355_blit_plan_rect_route": (C.c_int, [C.POINTER(PitchedPtr), C.POINTER(Dim3), C.POINTER(PitchedPtr),
                                              C.POINTER(Dim3), C.POINTER(Dim3), C.POINTER(Tuning), C.c_uint32,
                                              C.POINTER(RectPlan)]),
+    "mi355_blit_pages_book": (C.c_int, [C.c_uint32, C.c_uint32, C.c_uint32, C.POINTER(Book)]),
+    "mi355_blit_pages_create": (C.c_int, [C.c_void_p, C.POINTER(PagesDesc), C.POINTER(C.c_void_p)]),
+    "mi355_blit_pages_destroy": (C.c_int, [C.c_void_p]),
+    "mi355_blit_pages_reset": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "mi355_blit_pages_copy": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
+                                        C.c_uint32, C.c_void_p]),
+    "mi355_blit_pages_reserve": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]),
+    "mi355_blit_pages_fork": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]),
+    "mi355_blit_pages_free": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "mi355_blit_pages_compact": (C.c_int, [C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p]),
     "mi355_blit_signal_complete": (C.c_int, [C.c_void_p, C.c_uint64, C.c_void_p]),
     "mi355_blit_signal_stamp": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint32, C.c_void_p]),
     "mi355_blit_add_callback": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
@@ -249,6 +278,61 @@ class Blit:
     @property
     def stream(self):
         return self.lib.mi355_blit_stream(self.handle)
+
+
+def book_layout(num_pages, max_seqs, max_pages_per_seq):
+    """Where the parts of a book start, and its size, in 32-bit words."""
+    out = Book()
+    check(load().mi355_blit_pages_book(num_pages, max_seqs, max_pages_per_seq, C.byref(out)), "mi355_blit_pages_book")
+    return out
+
+
+class Pages:
+    """Owner of one mi355_blit_pages_t: the pages of a key/value cache, with a
+    book (max_seqs, max_pages_per_seq and the device address of its buffer) or, for
+    copies only, without.  planes: (base, pitch, row_bytes, runs) of each.  Methods
+    map 1:1 to the C ABI; lists are device addresses of int32."""
+
+    def __init__(self, blit, planes, num_pages, rows, max_seqs=0, max_pages_per_seq=0, book=None):
+        self.lib = load()
+        self.handle = None
+        array = (Plane * len(planes))(*[Plane(*p) for p in planes])
+        desc = PagesDesc(array, len(planes), num_pages, rows, max_seqs, max_pages_per_seq, 0, book)
+        p = C.c_void_p()
+        check(self.lib.mi355_blit_pages_create(blit.handle, C.byref(desc), C.byref(p)), "mi355_blit_pages_create")
+        self.handle = p
+
+    def close(self):
+        if self.handle:
+            st = self.lib.mi355_blit_pages_destroy(self.handle)
+            self.handle = None
+            check(st, "mi355_blit_pages_destroy")
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    def reset(self, stream=None):
+        return self.lib.mi355_blit_pages_reset(self.handle, stream)
+
+    def copy(self, dst_pages, src_pages, n, valid=None, src=None, route=ROUTE_DEVICE, stream=None):
+        """Pages of `src` (this pool if None) to pages of this pool."""
+        return self.lib.mi355_blit_pages_copy(self.handle, dst_pages, (src or self).handle, src_pages, valid, n, route,
+                                              stream)
+
+    def reserve(self, seqs, more, n, granted=None, stream=None):
+        return self.lib.mi355_blit_pages_reserve(self.handle, seqs, more, n, granted, stream)
+
+    def fork(self, parents, children, n, granted=None, stream=None):
+        return self.lib.mi355_blit_pages_fork(self.handle, parents, children, n, granted, stream)
+
+    def free(self, seqs, n, keep=None, stream=None):
+        return self.lib.mi355_blit_pages_free(self.handle, seqs, keep, n, stream)
+
+    def compact(self, max_moves, moves=None, stream=None):
+        return self.lib.mi355_blit_pages_compact(self.handle, max_moves, moves, stream)
 
 
 def plan_copy(dst, src, nbytes, num_cus=256, tuning=None, route=None):

@@ -18,6 +18,8 @@
 
 #include "blit_kernels.h"
 #include "blit_batch_host.h"
+#include "blit_pages.h"
+#include "blit_pages_kernels.h"
 #include "blit_plan.h"
 #include "blit_rect.h"
 #include "mi355_blit.h"
@@ -850,6 +852,219 @@ int mi355_blit_plan_rect_route(const mi355_pitched_ptr_t* dst, const mi355_dim3_
   out->store_policy = rp.store_policy;
   out->xcd_run = rp.xcd_run;
   return MI355_BLIT_SUCCESS;
+}
+
+// ---- pages of a key/value cache --------------------------------------------
+
+struct mi355_blit_pages {
+  mi355_blit* h = nullptr;
+  uint32_t num_pages = 0, rows = 0, n_planes = 0, segs = 0;
+  uint64_t page_bytes = 0;                  // over all planes
+  uint64_t (*planes)[2] = nullptr;          // row_bytes and runs of each, to compare two pools by
+  mi355::PageSegment* segs_dev = nullptr;
+  void* work_dev = nullptr;
+  bool has_book = false;
+  uint64_t book_words = 0;
+  mi355::BookPtrs book{};
+  mi355::PageMoveList moves{};
+};
+
+namespace {
+
+typedef void (*page_move_kernel_t)(PageMoveArgs);
+struct PageMoveVariant { unsigned nt_load, store; page_move_kernel_t fn; };
+#define MI355_PAGE_MOVE_ROW(L, S) {L, S, mi355_pages_move_l##L##_s##S},
+const PageMoveVariant kPageMoveVariants[] = {MI355_FOR_EACH_PAGE_MOVE_KERNEL(MI355_PAGE_MOVE_ROW)};
+
+// n moves, or the first *count of a list with room for n.
+int launch_page_moves(const mi355_blit_pages& to, const mi355_blit_pages& from, const int32_t* dst, const int32_t* src,
+                      const int32_t* valid, const uint32_t* count, uint64_t n, uint32_t route, hipStream_t s) {
+  const PageMovePlan p = plan_page_moves(n, to.segs, to.page_bytes, to.h->num_cus, route, kHostLinkMaxGrid);
+  page_move_kernel_t k = nullptr;
+  for (const PageMoveVariant& v : kPageMoveVariants)
+    if (v.nt_load == p.nt_load && v.store == p.store_policy) k = v.fn;
+  if (!k) return MI355_BLIT_ERROR;
+  const PageMoveArgs a{to.segs_dev, from.segs_dev, dst, src, valid, count, static_cast<uint32_t>(n), to.segs,
+                       magic_divisor(to.segs), to.num_pages, from.num_pages, to.rows, kMoveWaves, p.grid * kMoveWaves, 0};
+  hipLaunchKernelGGL(k, dim3(p.grid), dim3(p.wg_size), 0, s, a);
+  BLIT_HIP(hipGetLastError());
+  return MI355_BLIT_SUCCESS;
+}
+
+// What every call on a book checks before it looks at its lists.
+int check_book_call(const mi355_blit_pages* p, bool lists, size_t n) {
+  if (!p || !p->has_book || (n && !lists)) return MI355_BLIT_ERROR_INVALID_ARGUMENT;
+  if (n > MI355_BLIT_PAGES_MAX_LIST) return MI355_BLIT_ERROR_OUT_OF_RESOURCES;
+  return MI355_BLIT_SUCCESS;
+}
+
+}  // namespace
+
+int mi355_blit_pages_book(uint32_t num_pages, uint32_t max_seqs, uint32_t max_pages_per_seq, mi355_blit_book_t* out) {
+  return pages_book_layout(num_pages, max_seqs, max_pages_per_seq, out);
+}
+
+int mi355_blit_pages_create(mi355_blit_t* h, const mi355_blit_pages_desc_t* desc, mi355_blit_pages_t** out) {
+  if (!out) return MI355_BLIT_ERROR_INVALID_ARGUMENT;
+  *out = nullptr;
+  if (!h) return MI355_BLIT_ERROR_INVALID_ARGUMENT;
+  uint64_t segs = 0;
+  int rc = pages_check(desc, &segs);
+  if (rc != MI355_BLIT_SUCCESS) return rc;
+  std::lock_guard<std::mutex> g(h->lock);
+  DeviceScope scope(h->device);
+  if (scope.err != hipSuccess) return status_of(scope.err);
+  mi355_blit_pages* p = new (std::nothrow) mi355_blit_pages;
+  PageSegment* table = static_cast<PageSegment*>(std::malloc(segs * sizeof(PageSegment)));
+  if (p) p->planes = static_cast<uint64_t(*)[2]>(std::malloc(desc->n_planes * sizeof(*p->planes)));
+  hipError_t e = p && table && p->planes ? hipSuccess : hipErrorOutOfMemory;
+  if (e == hipSuccess) {
+    p->h = h;
+    p->num_pages = desc->num_pages;
+    p->rows = desc->rows;
+    p->n_planes = desc->n_planes;
+    p->segs = static_cast<uint32_t>(segs);
+    for (uint32_t i = 0; i < desc->n_planes; ++i) {
+      p->planes[i][0] = desc->planes[i].row_bytes;
+      p->planes[i][1] = desc->planes[i].runs;
+      p->page_bytes += plane_page_bytes(desc->planes[i], desc->rows);
+    }
+    pages_segments(*desc, table);
+    e = hipMalloc(reinterpret_cast<void**>(&p->segs_dev), segs * sizeof(PageSegment));
+  }
+  // through the default stream, and waited for
+  if (e == hipSuccess) e = hipMemcpy(p->segs_dev, table, segs * sizeof(PageSegment), hipMemcpyHostToDevice);
+  if (e == hipSuccess && desc->max_seqs) {
+    mi355_blit_book_t at;
+    rc = pages_book_layout(desc->num_pages, desc->max_seqs, desc->max_pages_per_seq, &at);
+    p->has_book = true;
+    p->book_words = at.words;
+    p->book = pages_book_ptrs(desc->book, at, desc->num_pages, desc->max_seqs, desc->max_pages_per_seq, desc->rows);
+    // lists of moves: an entry of a reservation, or a pair of a compaction
+    const uint64_t room = desc->num_pages > 2 * kMaxList ? desc->num_pages / 2 : kMaxList;
+    const uint64_t words = 64 + 3 * room + desc->num_pages;
+    if (rc == MI355_BLIT_SUCCESS) e = hipMalloc(&p->work_dev, words * sizeof(int32_t));
+    if (rc == MI355_BLIT_SUCCESS && e == hipSuccess) {
+      int32_t* w = static_cast<int32_t*>(p->work_dev);
+      p->moves = {w + 64, w + 64 + room, w + 64 + 2 * room, w + 64 + 3 * room, reinterpret_cast<uint32_t*>(w)};
+    }
+  }
+  std::free(table);
+  if (rc == MI355_BLIT_SUCCESS && e == hipSuccess) {
+    *out = p;
+    return MI355_BLIT_SUCCESS;
+  }
+  if (p) {
+    if (p->segs_dev) (void)hipFree(p->segs_dev);
+    if (p->work_dev) (void)hipFree(p->work_dev);
+    std::free(p->planes);
+    delete p;
+  }
+  return rc != MI355_BLIT_SUCCESS ? rc : status_of(e);
+}
+
+int mi355_blit_pages_destroy(mi355_blit_pages_t* p) {
+  if (!p) return MI355_BLIT_ERROR_INVALID_ARGUMENT;
+  {
+    std::lock_guard<std::mutex> g(p->h->lock);
+    DeviceScope scope(p->h->device);
+    if (scope.err != hipSuccess) return status_of(scope.err);
+    // commands may be on any stream; memory that they still use is not freed
+    BLIT_HIP(hipDeviceSynchronize());
+    (void)hipFree(p->segs_dev);
+    if (p->work_dev) (void)hipFree(p->work_dev);
+  }
+  std::free(p->planes);
+  delete p;
+  return MI355_BLIT_SUCCESS;
+}
+
+int mi355_blit_pages_reset(mi355_blit_pages_t* p, void* stream) {
+  if (!p || !p->has_book) return MI355_BLIT_ERROR_INVALID_ARGUMENT;
+  std::lock_guard<std::mutex> g(p->h->lock);
+  DeviceScope scope(p->h->device);
+  if (scope.err != hipSuccess) return status_of(scope.err);
+  const PageResetArgs a{p->book, p->book_words};
+  hipLaunchKernelGGL(mi355_pages_reset, dim3(static_cast<uint32_t>((p->book_words + 255) / 256)), dim3(256), 0,
+                     stream ? static_cast<hipStream_t>(stream) : p->h->stream, a);
+  BLIT_HIP(hipGetLastError());
+  return MI355_BLIT_SUCCESS;
+}
+
+int mi355_blit_pages_copy(mi355_blit_pages_t* dst, const int32_t* dst_pages, mi355_blit_pages_t* src,
+                          const int32_t* src_pages, const int32_t* valid_rows, size_t n, uint32_t route,
+                          void* stream) {
+  if (!dst || !src || route > MI355_BLIT_ROUTE_DEVICE_TO_HOST || (n && (!dst_pages || !src_pages)))
+    return MI355_BLIT_ERROR_INVALID_ARGUMENT;
+  if (dst != src && (dst->h->device != src->h->device || dst->rows != src->rows || dst->n_planes != src->n_planes ||
+                     std::memcmp(dst->planes, src->planes, dst->n_planes * sizeof(*dst->planes)) != 0))
+    return MI355_BLIT_ERROR_INVALID_ARGUMENT;
+  if (n == 0) return MI355_BLIT_SUCCESS;
+  if (n > 0xffffffffull / dst->segs) return MI355_BLIT_ERROR_OUT_OF_RESOURCES;
+  std::lock_guard<std::mutex> g(dst->h->lock);
+  DeviceScope scope(dst->h->device);
+  if (scope.err != hipSuccess) return status_of(scope.err);
+  return launch_page_moves(*dst, *src, dst_pages, src_pages, valid_rows, nullptr, n, route,
+                           stream ? static_cast<hipStream_t>(stream) : dst->h->stream);
+}
+
+int mi355_blit_pages_reserve(mi355_blit_pages_t* p, const int32_t* seqs, const int32_t* more, size_t n,
+                             int32_t* granted, void* stream) {
+  const int rc = check_book_call(p, seqs && more, n);
+  if (rc != MI355_BLIT_SUCCESS || n == 0) return rc;
+  std::lock_guard<std::mutex> g(p->h->lock);
+  DeviceScope scope(p->h->device);
+  if (scope.err != hipSuccess) return status_of(scope.err);
+  hipStream_t s = stream ? static_cast<hipStream_t>(stream) : p->h->stream;
+  const PageReserveArgs a{p->book, p->moves, seqs, more, granted, static_cast<uint32_t>(n), 0};
+  hipLaunchKernelGGL(mi355_pages_reserve, dim3(1), dim3(1024), 0, s, a);
+  BLIT_HIP(hipGetLastError());
+  return launch_page_moves(*p, *p, p->moves.dst, p->moves.src, p->moves.valid, p->moves.count,
+                           n < p->num_pages ? n : p->num_pages, MI355_BLIT_ROUTE_DEVICE, s);
+}
+
+int mi355_blit_pages_fork(mi355_blit_pages_t* p, const int32_t* parents, const int32_t* children, size_t n,
+                          int32_t* granted, void* stream) {
+  const int rc = check_book_call(p, parents && children, n);
+  if (rc != MI355_BLIT_SUCCESS || n == 0) return rc;
+  std::lock_guard<std::mutex> g(p->h->lock);
+  DeviceScope scope(p->h->device);
+  if (scope.err != hipSuccess) return status_of(scope.err);
+  const PageForkArgs a{p->book, parents, children, granted, static_cast<uint32_t>(n), 0};
+  hipLaunchKernelGGL(mi355_pages_fork, dim3(static_cast<uint32_t>(n)), dim3(256), 0,
+                     stream ? static_cast<hipStream_t>(stream) : p->h->stream, a);
+  BLIT_HIP(hipGetLastError());
+  return MI355_BLIT_SUCCESS;
+}
+
+int mi355_blit_pages_free(mi355_blit_pages_t* p, const int32_t* seqs, const int32_t* keep, size_t n, void* stream) {
+  const int rc = check_book_call(p, seqs != nullptr, n);
+  if (rc != MI355_BLIT_SUCCESS || n == 0) return rc;
+  std::lock_guard<std::mutex> g(p->h->lock);
+  DeviceScope scope(p->h->device);
+  if (scope.err != hipSuccess) return status_of(scope.err);
+  const PageFreeArgs a{p->book, seqs, keep, static_cast<uint32_t>(n), 0};
+  hipLaunchKernelGGL(mi355_pages_free, dim3(static_cast<uint32_t>(n)), dim3(256), 0,
+                     stream ? static_cast<hipStream_t>(stream) : p->h->stream, a);
+  BLIT_HIP(hipGetLastError());
+  return MI355_BLIT_SUCCESS;
+}
+
+int mi355_blit_pages_compact(mi355_blit_pages_t* p, uint32_t max_moves, int32_t* moves, void* stream) {
+  if (!p || !p->has_book) return MI355_BLIT_ERROR_INVALID_ARGUMENT;
+  // a hole for each page that moves
+  const uint32_t most = max_moves < p->num_pages / 2 ? max_moves : p->num_pages / 2;
+  if (most == 0) return MI355_BLIT_SUCCESS;
+  std::lock_guard<std::mutex> g(p->h->lock);
+  DeviceScope scope(p->h->device);
+  if (scope.err != hipSuccess) return status_of(scope.err);
+  hipStream_t s = stream ? static_cast<hipStream_t>(stream) : p->h->stream;
+  const PageCompactArgs a{p->book, p->moves, moves, most, 0};
+  hipLaunchKernelGGL(mi355_pages_compact_plan, dim3(1), dim3(1024), 0, s, a);
+  hipLaunchKernelGGL(mi355_pages_compact_apply, dim3((most + 255) / 256), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(mi355_pages_compact_tables, dim3(p->book.max_seqs), dim3(256), 0, s, a);
+  BLIT_HIP(hipGetLastError());
+  return launch_page_moves(*p, *p, p->moves.dst, p->moves.src, nullptr, p->moves.count, most, MI355_BLIT_ROUTE_DEVICE, s);
 }
 
 namespace {

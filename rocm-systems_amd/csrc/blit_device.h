@@ -16,6 +16,7 @@
 #include <stdint.h>
 
 #include "blit_args.h"
+#include "blit_pages.h"
 
 #define MI355_DEVICE __device__ __forceinline__
 // A kernel entry point for workgroups of up to `max_wg` work-items.
@@ -176,6 +177,62 @@ MI355_DEVICE uint32_t ld_uniform_u32(const uint32_t* p) {
   return *(ConstPtr)(p);
 #pragma clang diagnostic pop
 }
+
+// A segment of a page, at an address that is the same for every lane, through
+// the constant address space like a record.
+MI355_DEVICE PageSegment ld_uniform_segment(const PageSegment* p) {
+  typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
+  typedef const u32x8 __attribute__((address_space(4))) * ConstPtr;
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Wold-style-cast"
+  const u32x8 v = *(ConstPtr)(p);
+#pragma clang diagnostic pop
+  PageSegment s;
+  __builtin_memcpy(&s, &v, sizeof(s));
+  return s;
+}
+
+// Words that other workgroups of the same launch change too: read, and changed
+// at once, where every XCD sees them (agent scope).  The changes return the old value.
+MI355_DEVICE uint32_t ld_agent_u32(const uint32_t* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+MI355_DEVICE int32_t add_agent_i32(int32_t* p, int32_t v) {
+  return __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+MI355_DEVICE int32_t min_agent_i32(int32_t* p, int32_t v) {
+  return __hip_atomic_fetch_min(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+MI355_DEVICE uint32_t or_agent_u32(uint32_t* p, uint32_t v) {
+  return __hip_atomic_fetch_or(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+MI355_DEVICE uint32_t and_agent_u32(uint32_t* p, uint32_t v) {
+  return __hip_atomic_fetch_and(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// Returns when the wave's loads, stores and atomics have been performed.
+MI355_DEVICE void wait_for_memory() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Changes of words in LDS; they return the old value.
+MI355_DEVICE uint32_t lds_compare_swap(uint32_t* p, uint32_t expected, uint32_t v) {
+  __hip_atomic_compare_exchange_strong(p, &expected, v, __ATOMIC_RELAXED, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  return expected;
+}
+MI355_DEVICE uint32_t lds_add(uint32_t* p, uint32_t v) {
+  return __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+MI355_DEVICE uint32_t lds_min(uint32_t* p, uint32_t v) {
+  return __hip_atomic_fetch_min(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+MI355_DEVICE uint32_t lds_max(uint32_t* p, uint32_t v) {
+  return __hip_atomic_fetch_max(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+MI355_DEVICE uint32_t lds_or(uint32_t* p, uint32_t v) {
+  return __hip_atomic_fetch_or(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+
+MI355_DEVICE unsigned popcount32(uint32_t v) { return __popc(v); }
+// Index of the lowest bit that is set; v is not 0.
+MI355_DEVICE unsigned lowest_bit(uint32_t v) { return static_cast<unsigned>(__ffs(static_cast<int>(v))) - 1; }
 
 // Keeps the compiler from dropping a load whose value is not used.
 MI355_DEVICE void keep_alive(unsigned v) { asm volatile("" ::"v"(v)); }

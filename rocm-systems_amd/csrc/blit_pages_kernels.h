@@ -1,0 +1,518 @@
+// Kernels for the pages of a key/value cache (blit_pages.h has their arguments).
+//
+// What they have in common: lists, tables and counts stay on the device, so a
+// call needs no answer from it before the next one can be submitted, and all of
+// them can be recorded into a graph.  No workgroup waits for another; what one
+// launch decides for many workgroups, the next launch reads.  Numbers of pages
+// and of sequences come from memory that the caller can write, so every one of
+// them is checked before it becomes an address.
+#ifndef MI355_BLIT_PAGES_KERNELS_H_
+#define MI355_BLIT_PAGES_KERNELS_H_
+
+#include "blit_kernels.h"
+#include "blit_pages.h"
+
+namespace mi355 {
+
+// ---------------------------------------------------------------------------
+// Moves.  One wave moves one segment (4 KiB: four 16-byte loads of each lane
+// in flight before the first store).  Bound by memory: 2 bytes of traffic for
+// each byte of the pages that are named, nothing else.
+// ---------------------------------------------------------------------------
+
+// A page of several runs of which only the first rows are moved: the bytes
+// whose place in their run is below `limit`.  A vector may lie across the end
+// of the rows or of a run; such a one goes byte by byte.
+template <bool NTL, int ST>
+MI355_DEVICE void move_cut_runs(uint8_t* d, const uint8_t* s, const PageSegment& g, unsigned limit, unsigned lane) {
+  for (unsigned at = 16 * lane; at < g.bytes; at += 16 * kWave) {
+    const unsigned in_run = (g.offset + at) % g.run_bytes;
+    const unsigned left = g.bytes - at;
+    if (left >= 16 && in_run + 16 <= limit) {
+      st_v4_any<ST>(reinterpret_cast<uintptr_t>(d + at), ld_v4_any<NTL>(s + at));
+    } else if (in_run < limit || in_run + 16 > g.run_bytes) {
+      const unsigned n = left < 16 ? left : 16;
+      for (unsigned b = 0; b < n; ++b)
+        if ((g.offset + at + b) % g.run_bytes < limit) st_u8(d + at + b, ld_u8(s + at + b));
+    }
+  }
+}
+
+template <bool NTL, int ST>
+MI355_DEVICE void move_segment(uint8_t* d, const uint8_t* s, const PageSegment& g, unsigned valid, unsigned rows,
+                               unsigned lane) {
+  unsigned bytes = g.bytes;
+  if (valid < rows) {
+    const unsigned limit = valid * g.row_bytes;
+    if (g.run_bytes) {
+      move_cut_runs<NTL, ST>(d, s, g, limit, lane);
+      return;
+    }
+    if (limit <= g.offset) return;
+    if (limit - g.offset < bytes) bytes = limit - g.offset;
+  }
+  const unsigned vecs = bytes / 16;
+  v4u x[kPageUnroll];
+#pragma unroll
+  for (unsigned u = 0; u < kPageUnroll; ++u)
+    if (lane + u * kWave < vecs) x[u] = ld_v4_any<NTL>(s + 16 * (lane + u * kWave));
+#pragma unroll
+  for (unsigned u = 0; u < kPageUnroll; ++u)
+    if (lane + u * kWave < vecs) st_v4_any<ST>(reinterpret_cast<uintptr_t>(d + 16 * (lane + u * kWave)), x[u]);
+  const unsigned tail = bytes & 15;
+  if (lane < tail) st_u8(d + 16 * vecs + lane, ld_u8(s + 16 * vecs + lane));
+}
+
+template <bool NTL, int ST>
+MI355_DEVICE void page_move_body(const PageMoveArgs& a) {
+  const unsigned lane = thread_in_workgroup() & (kWave - 1);
+  uint32_t n = a.n;
+  if (a.count) {
+    const uint32_t found = ld_uniform_u32(a.count);
+    if (found < n) n = found;
+  }
+  // n * segs fits in 32 bits, and so does what a wave adds to get past it
+  // (checked on the host): 64 bits only for the sum
+  const uint64_t total = static_cast<uint64_t>(n) * a.segs;
+  for (uint64_t w = global_wave(a.waves_per_wg); w < total; w += a.n_waves) {
+    const uint32_t move = div_magic(static_cast<uint32_t>(w), a.magic_segs);
+    const uint32_t seg = static_cast<uint32_t>(w) - move * a.segs;
+    const uint32_t to = ld_uniform_u32(reinterpret_cast<const uint32_t*>(a.dst + move));
+    const uint32_t from = ld_uniform_u32(reinterpret_cast<const uint32_t*>(a.src + move));
+    uint32_t valid = a.rows;
+    if (a.valid) {
+      const int32_t v = static_cast<int32_t>(ld_uniform_u32(reinterpret_cast<const uint32_t*>(a.valid + move)));
+      if (v < static_cast<int32_t>(a.rows)) valid = v > 0 ? v : 0;
+    }
+    // a negative number is a large unsigned one
+    if (to >= a.dst_pages || from >= a.src_pages || valid == 0) continue;
+    const PageSegment d = ld_uniform_segment(a.dst_segs + seg);
+    const PageSegment s = ld_uniform_segment(a.src_segs + seg);
+    move_segment<NTL, ST>(d.base + to * d.pitch, s.base + from * s.pitch, s, valid, a.rows, lane);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The book.
+// ---------------------------------------------------------------------------
+
+// Pages that `tokens` tokens take.
+MI355_DEVICE uint32_t pages_held(uint32_t tokens, const BookPtrs& b) {
+  return div_magic(tokens, b.magic_rows) + (tokens - div_magic(tokens, b.magic_rows) * b.rows ? 1 : 0);
+}
+
+// A tile of the free bits: four words for each of the 1024 lanes.  Bits of
+// pages that do not exist are taken as 0 whatever the buffer holds.
+constexpr uint32_t kTileWords = 4 * 1024;
+constexpr uint32_t kTilePages = 32 * kTileWords;
+
+struct BitTile {
+  uint32_t word[4];
+};
+
+MI355_DEVICE BitTile load_bits(const BookPtrs& b, uint32_t tile) {
+  BitTile t;
+  const uint32_t w = tile * kTileWords + 4 * thread_in_workgroup();
+#pragma unroll
+  for (unsigned k = 0; k < 4; ++k) t.word[k] = 0;
+  if (w * 32 < b.num_pages) {
+    const v4u v = ld_v4<false>(reinterpret_cast<const v4u_a4*>(b.bits + w));
+    t.word[0] = v.x, t.word[1] = v.y, t.word[2] = v.z, t.word[3] = v.w;
+#pragma unroll
+    for (unsigned k = 0; k < 4; ++k) {
+      const uint32_t first = 32 * (w + k);
+      if (first >= b.num_pages) t.word[k] = 0;
+      else if (b.num_pages - first < 32) t.word[k] &= (1u << (b.num_pages - first)) - 1;
+    }
+  }
+  return t;
+}
+
+MI355_DEVICE uint32_t count_bits(const BitTile& t) {
+  return popcount32(t.word[0]) + popcount32(t.word[1]) + popcount32(t.word[2]) + popcount32(t.word[3]);
+}
+
+// A table in LDS that finds equal keys among the 1024 entries of a round: open
+// addressing over twice as many slots, so that a free one is always found.
+constexpr uint32_t kSlots = 2048;
+constexpr uint32_t kNoKey = ~0u;
+
+MI355_DEVICE uint32_t hash_slot(uint32_t* keys, uint32_t key) {
+  uint32_t at = (key * 2654435761u) >> 21;  // 11 bits
+  for (;;) {
+    const uint32_t was = lds_compare_swap(keys + at, kNoKey, key);
+    if (was == kNoKey || was == key) return at;
+    at = (at + 1) & (kSlots - 1);
+  }
+}
+
+// Room for new tokens.  One workgroup of 1024 lanes takes the entries 1024 at
+// a time: which of them name a sequence first (a table in LDS, and a bit for each sequence
+// that an earlier round named), which of them have to copy a last page that
+// others hold as well, how many pages each needs, and from the free bits
+// which pages those are: the k-th lowest free page goes to the entry whose
+// share of the running sum of needs k falls into, so that the result is that of
+// taking the entries one by one.
+//
+// Bound by latency: a chain of dependent loads (entry, length, last page,
+// its count, free bits) and a dozen barriers.
+MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
+  constexpr uint32_t kIds = 2048;
+  MI355_LDS uint32_t scan_a[16], scan_b[16];
+  MI355_LDS uint32_t keys[kSlots], first[kSlots], asked[kSlots];
+  MI355_LDS uint32_t seen[kMaxSeqs / 32];
+  MI355_LDS uint32_t start[1024], who[1024], slot_of[1024], tail_of[1024], fill_of[1024];
+  MI355_LDS uint32_t ids[kIds];
+  MI355_LDS uint32_t any_shared, any_refused, granted_pages, n_moves;
+  const BookPtrs& b = a.book;
+  const uint32_t t = thread_in_workgroup();
+  const uint32_t n_tiles = (b.num_pages + kTilePages - 1) / kTilePages;
+
+  for (uint32_t k = t; k < kMaxSeqs / 32; k += 1024) seen[k] = 0;
+  if (t == 0) n_moves = 0;
+  uint32_t tile = 0;     // no free page in front of this tile
+  bool stopped = false;  // the same in all lanes
+  for (uint32_t base = 0; base < a.n; base += 1024) {
+    const uint32_t i = base + t;
+    if (stopped) {
+      if (i < a.n && a.granted) st_obj(a.granted + i, 0);
+      continue;
+    }
+    for (uint32_t k = t; k < kSlots; k += 1024) keys[k] = kNoKey, first[k] = ~0u;
+    if (t == 0) any_shared = 0, any_refused = 0, granted_pages = 0;
+    workgroup_barrier();
+
+    const uint32_t s = i < a.n ? static_cast<uint32_t>(ld_obj(a.seqs + i)) : ~0u;
+    const int32_t more = i < a.n ? ld_obj(a.add + i) : 0;
+    const bool named = s < b.max_seqs;
+    uint32_t slot = 0, tokens = 0;
+    bool again = false;
+    if (named) {
+      again = seen[s / 32] >> (s % 32) & 1;
+      slot = hash_slot(keys, s);
+      lds_min(first + slot, t);
+      tokens = ld_obj(b.lengths + s);
+    }
+    workgroup_barrier();
+    if (named) {
+      again = again || first[slot] != t;
+      lds_or(seen + s / 32, 1u << (s % 32));
+    }
+    // both below 2^31, so the sum is below 2^32
+    const uint32_t old_pages = pages_held(tokens, b);
+    const uint32_t new_pages = more >= 0 ? pages_held(tokens + more, b) : 0;
+    bool ok = named && !again && more >= 0 && static_cast<int32_t>(tokens) >= 0 && new_pages <= b.width;
+    const uint32_t fill = tokens - div_magic(tokens, b.magic_rows) * b.rows;
+    bool shared = false;
+    uint32_t tail = 0, holders = 0;
+    if (ok && more > 0 && fill != 0) {
+      tail = ld_obj(b.tables + static_cast<uint64_t>(s) * b.width + old_pages - 1);
+      if (tail < b.num_pages) {
+        holders = ld_agent_u32(reinterpret_cast<const uint32_t*>(b.refs + tail));
+        shared = static_cast<int32_t>(holders) > 1;
+      } else {
+        ok = false;  // not a page
+      }
+    }
+    if (shared) any_shared = 1;
+    workgroup_barrier();
+    bool copies = shared;
+    if (any_shared) {
+      // With as many askers as holders, the last of them finds the page its own.
+      for (uint32_t k = t; k < kSlots; k += 1024) keys[k] = kNoKey, first[k] = 0, asked[k] = 0;
+      workgroup_barrier();
+      if (shared) {
+        slot = hash_slot(keys, tail);
+        lds_max(first + slot, t);
+        lds_add(asked + slot, 1);
+      }
+      workgroup_barrier();
+      copies = shared && !(asked[slot] == holders && first[slot] == t);
+    }
+    uint32_t need = ok ? new_pages - old_pages + (copies ? 1 : 0) : 0;
+    // more than the pool has is as good as one more: the sum over 1024 entries
+    // stays below 2^32 (kMaxPages)
+    if (need > b.num_pages) need = b.num_pages + 1;
+    uint32_t total;
+    const uint32_t before = block_scan_1024(need, scan_a, &total);
+
+    // how many of them there are
+    uint32_t found = 0;
+    for (uint32_t k = tile; k < n_tiles && found < total; ++k) {
+      uint32_t here;
+      block_scan_1024(count_bits(load_bits(b, k)), scan_b, &here);
+      found += here;
+      workgroup_barrier();
+    }
+    const bool granted = ok && before + need <= found;
+    if (ok && !granted) any_refused = 1;
+    if (granted) lds_max(&granted_pages, before + need);
+    start[t] = before;
+    who[t] = s | (copies ? 1u << 31 : 0);
+    slot_of[t] = old_pages - (copies ? 1 : 0);
+    tail_of[t] = tail;
+    fill_of[t] = fill;
+    workgroup_barrier();
+    stopped = any_refused != 0;
+    const uint32_t wanted = granted_pages;
+
+    // the pages, lowest first
+    uint32_t done = 0;
+    while (done < wanted) {
+      BitTile bits = load_bits(b, tile);
+      uint32_t here;
+      uint32_t rank = block_scan_1024(count_bits(bits), scan_b, &here);
+      workgroup_barrier();
+      const uint32_t take = here < wanted - done ? here : wanted - done;
+      const uint32_t w = tile * kTileWords + 4 * t;
+      unsigned k = 0;
+      bool changed = false;
+      for (uint32_t round = 0; round < take; round += kIds) {
+        const uint32_t end = take - round < kIds ? take : round + kIds;
+        while (k < 4 && rank < end) {
+          if (bits.word[k] == 0) {
+            ++k;
+            continue;
+          }
+          ids[rank - round] = 32 * (w + k) + lowest_bit(bits.word[k]);
+          bits.word[k] &= bits.word[k] - 1;
+          changed = true;
+          ++rank;
+        }
+        workgroup_barrier();
+        for (uint32_t q = round + t; q < end; q += 1024) {
+          const uint32_t page = ids[q - round];
+          const uint32_t nth = done + q;
+          uint32_t e = 0;  // the last entry that starts at or in front of nth
+#pragma unroll
+          for (uint32_t step = 512; step >= 1; step >>= 1)
+            if (start[e + step] <= nth) e += step;
+          const uint32_t seq = who[e] & 0x7fffffffu;
+          const uint32_t j = nth - start[e];
+          st_obj(b.tables + static_cast<uint64_t>(seq) * b.width + slot_of[e] + j, static_cast<int32_t>(page));
+          st_obj(b.refs + page, 1);
+          if (j == 0 && who[e] >> 31) {
+            const uint32_t m = lds_add(&n_moves, 1);
+            st_obj(a.moves.src + m, static_cast<int32_t>(tail_of[e]));
+            st_obj(a.moves.dst + m, static_cast<int32_t>(page));
+            st_obj(a.moves.valid + m, static_cast<int32_t>(fill_of[e]));
+            add_agent_i32(b.refs + tail_of[e], -1);
+          }
+        }
+        workgroup_barrier();
+      }
+      if (changed) {
+        // words behind the last page are not written
+#pragma unroll
+        for (unsigned c = 0; c < 4; ++c)
+          if (32 * (w + c) < b.num_pages) st_u32(b.bits + w + c, bits.word[c]);
+      }
+      done += take;
+      if (done < wanted) ++tile;
+    }
+    if (granted && more > 0) st_obj(b.lengths + s, static_cast<int32_t>(tokens + more));
+    if (i < a.n && a.granted) st_obj(a.granted + i, granted ? 1 : 0);
+    // the next round reads counts and bits that this one wrote
+    wait_for_memory();
+    workgroup_barrier();
+  }
+  if (t == 0) st_obj(a.moves.count, n_moves);
+}
+
+// A sequence that holds its parent's pages.  A workgroup of 256 lanes for each
+// entry; the list is read by every one of them (it is short and in L2), so that
+// no entry depends on what another has already written: a child that an
+// earlier entry names too is left alone, and so is one whose parent is named
+// as a child.  Bound by the atomic additions.
+MI355_DEVICE void page_fork_body(const PageForkArgs& a) {
+  MI355_LDS uint32_t refused;
+  const BookPtrs& b = a.book;
+  const uint32_t t = thread_in_workgroup();
+  const uint32_t i = workgroup_index();
+  const uint32_t parent = static_cast<uint32_t>(ld_obj(a.parents + i));
+  const uint32_t child = static_cast<uint32_t>(ld_obj(a.children + i));
+  if (t == 0) refused = 0;
+  workgroup_barrier();
+  const bool in_range = parent < b.max_seqs && child < b.max_seqs;
+  if (in_range) {
+    bool bad = ld_obj(b.lengths + child) != 0;
+    for (uint32_t k = t; k < a.n; k += 256) {
+      const uint32_t c = static_cast<uint32_t>(ld_obj(a.children + k));
+      if (c == parent || (c == child && k < i)) bad = true;
+    }
+    if (bad) refused = 1;
+  }
+  workgroup_barrier();
+  const bool made = in_range && !refused;
+  if (made) {
+    const uint32_t tokens = ld_obj(b.lengths + parent);
+    uint32_t held = pages_held(tokens, b);
+    if (held > b.width) held = 0;  // not a length
+    const int32_t* from = b.tables + static_cast<uint64_t>(parent) * b.width;
+    int32_t* to = b.tables + static_cast<uint64_t>(child) * b.width;
+    for (uint32_t j = t; j < held; j += 256) {
+      const int32_t page = ld_obj(from + j);
+      st_obj(to + j, page);
+      if (static_cast<uint32_t>(page) < b.num_pages) add_agent_i32(b.refs + page, 1);
+    }
+    if (t == 0 && held) st_obj(b.lengths + child, static_cast<int32_t>(tokens));
+  }
+  if (t == 0 && a.granted) st_obj(a.granted + i, made ? 1 : 0);
+}
+
+// The end of a sequence, or of its tokens from `keep` on.  A workgroup of 256
+// lanes for each entry; lane 0 takes the sequence's tokens with an atomic
+// minimum, so that of two entries for one sequence each gives back what the
+// other has not.  Bound by the atomics.
+MI355_DEVICE void page_free_body(const PageFreeArgs& a) {
+  MI355_LDS uint32_t before;
+  const BookPtrs& b = a.book;
+  const uint32_t t = thread_in_workgroup();
+  const uint32_t i = workgroup_index();
+  const uint32_t s = static_cast<uint32_t>(ld_obj(a.seqs + i));
+  const int32_t keep = a.keep ? ld_obj(a.keep + i) : 0;
+  if (s >= b.max_seqs || keep < 0) return;
+  if (t == 0) before = static_cast<uint32_t>(min_agent_i32(b.lengths + s, keep));
+  workgroup_barrier();
+  const uint32_t was = before;
+  if (static_cast<int32_t>(was) <= keep) return;
+  uint32_t end = pages_held(was, b);
+  if (end > b.width) end = b.width;
+  const int32_t* table = b.tables + static_cast<uint64_t>(s) * b.width;
+  for (uint32_t j = pages_held(keep, b) + t; j < end; j += 256) {
+    const uint32_t page = static_cast<uint32_t>(ld_obj(table + j));
+    if (page >= b.num_pages) continue;
+    if (add_agent_i32(b.refs + page, -1) == 1) or_agent_u32(b.bits + page / 32, 1u << (page % 32));
+  }
+}
+
+// Compaction.  With L pages in use, a page below L that is free is a hole and a
+// page from L on that is in use has to move; there are as many of the one as
+// of the other.  The i-th hole from below takes the i-th page from above, as far as the
+// caller's budget goes.  One workgroup of 1024 lanes makes the two lists from
+// the free bits (first how many pages are in use, then their ranks).
+MI355_DEVICE void page_compact_plan_body(const PageCompactArgs& a) {
+  MI355_LDS uint32_t scan_a[16], scan_b[16];
+  const BookPtrs& b = a.book;
+  const uint32_t t = thread_in_workgroup();
+  const uint32_t n_tiles = (b.num_pages + kTilePages - 1) / kTilePages;
+  uint32_t free_pages = 0;
+  for (uint32_t k = 0; k < n_tiles; ++k) {
+    uint32_t here;
+    block_scan_1024(count_bits(load_bits(b, k)), scan_a, &here);
+    free_pages += here;
+    workgroup_barrier();
+  }
+  const uint32_t live = b.num_pages - free_pages;
+  uint32_t holes = 0, movers = 0;
+  for (uint32_t k = 0; k < n_tiles; ++k) {
+    const BitTile bits = load_bits(b, k);
+    BitTile low, high;
+#pragma unroll
+    for (unsigned c = 0; c < 4; ++c) {
+      const uint32_t page = 32 * (k * kTileWords + 4 * t + c);
+      // pages of this word below `live`, and pages that exist
+      const uint32_t below = page >= live ? 0 : live - page >= 32 ? ~0u : (1u << (live - page)) - 1;
+      const uint32_t exist = page >= b.num_pages ? 0 : b.num_pages - page >= 32 ? ~0u : (1u << (b.num_pages - page)) - 1;
+      low.word[c] = bits.word[c] & below;
+      high.word[c] = ~bits.word[c] & ~below & exist;
+    }
+    uint32_t here;
+    uint32_t rank = holes + block_scan_1024(count_bits(low), scan_a, &here);
+    holes += here;
+#pragma unroll
+    for (unsigned c = 0; c < 4; ++c)
+      for (uint32_t m = low.word[c]; m; m &= m - 1, ++rank)
+        if (rank < a.max_moves)
+          st_obj(a.moves.dst + rank, static_cast<int32_t>(32 * (k * kTileWords + 4 * t + c) + lowest_bit(m)));
+    // every hole is below every page that moves: `holes` is final where one is met
+    rank = movers + block_scan_1024(count_bits(high), scan_b, &here);
+    movers += here;
+#pragma unroll
+    for (unsigned c = 0; c < 4; ++c)
+      for (uint32_t m = high.word[c]; m; m &= m - 1, ++rank) {
+        const uint32_t from_top = holes - 1 - rank;
+        if (from_top < a.max_moves)
+          st_obj(a.moves.src + from_top, static_cast<int32_t>(32 * (k * kTileWords + 4 * t + c) + lowest_bit(m)));
+      }
+    workgroup_barrier();
+  }
+  if (t == 0) {
+    const uint32_t n = holes < a.max_moves ? holes : a.max_moves;
+    st_obj(a.moves.count, n);
+    st_obj(b.head, static_cast<int32_t>(n));
+  }
+}
+
+// The counts and free bits of the pages that move, a lane for each.
+MI355_DEVICE void page_compact_apply_body(const PageCompactArgs& a) {
+  const BookPtrs& b = a.book;
+  const uint32_t n = ld_uniform_u32(a.moves.count);
+  const uint32_t k = workgroup_index() * 256 + thread_in_workgroup();
+  if (k >= n) return;
+  const uint32_t from = ld_obj(a.moves.src + k), to = ld_obj(a.moves.dst + k);
+  st_obj(b.refs + to, ld_obj(b.refs + from));
+  st_obj(b.refs + from, 0);
+  or_agent_u32(b.bits + from / 32, 1u << (from % 32));
+  and_agent_u32(b.bits + to / 32, ~(1u << (to % 32)));
+  st_obj(a.moves.remap + from, static_cast<int32_t>(to));
+  if (a.out) {
+    st_obj(a.out + 2 * static_cast<uint64_t>(k), static_cast<int32_t>(from));
+    st_obj(a.out + 2 * static_cast<uint64_t>(k) + 1, static_cast<int32_t>(to));
+  }
+}
+
+// The tables, a workgroup of 256 lanes for each sequence.  The pages that moved
+// are the highest ones, so every held page from the lowest of them on has moved.
+MI355_DEVICE void page_compact_tables_body(const PageCompactArgs& a) {
+  const BookPtrs& b = a.book;
+  const uint32_t n = ld_uniform_u32(a.moves.count);
+  if (n == 0) return;
+  const uint32_t lowest = ld_uniform_u32(reinterpret_cast<const uint32_t*>(a.moves.src + n - 1));
+  const uint32_t s = workgroup_index();
+  uint32_t held = pages_held(ld_obj(b.lengths + s), b);
+  if (held > b.width) held = 0;
+  int32_t* table = b.tables + static_cast<uint64_t>(s) * b.width;
+  for (uint32_t j = thread_in_workgroup(); j < held; j += 256) {
+    const uint32_t page = static_cast<uint32_t>(ld_obj(table + j));
+    if (page >= lowest && page < b.num_pages) st_obj(table + j, ld_obj(a.moves.remap + page));
+  }
+}
+
+// An empty book: no tokens, no holders, every page free, no table entry.
+MI355_DEVICE void page_reset_body(const PageResetArgs& a) {
+  const BookPtrs& b = a.book;
+  const int64_t bits_at = reinterpret_cast<int32_t*>(b.bits) - b.head;
+  const int64_t tables_at = b.tables - b.head;
+  const uint64_t i = static_cast<uint64_t>(workgroup_index()) * 256 + thread_in_workgroup();
+  if (i >= a.words) return;
+  uint32_t v = 0;
+  if (static_cast<int64_t>(i) >= tables_at) {
+    v = ~0u;
+  } else if (static_cast<int64_t>(i) >= bits_at) {
+    const uint64_t page = 32 * (i - bits_at);
+    if (page < b.num_pages) v = b.num_pages - page >= 32 ? ~0u : (1u << (b.num_pages - page)) - 1;
+  }
+  st_obj(b.head + i, static_cast<int32_t>(v));
+}
+
+}  // namespace mi355
+
+// Entry points, named as those of blit_kernels.h:
+//   mi355_pages_move_l<nt loads>_s<store policy>
+#define MI355_FOR_EACH_PAGE_MOVE_KERNEL(X) X(0, 0) X(1, 2) X(0, 3) X(1, 3)
+#define MI355_DEFINE_PAGE_MOVE(L, S)                                                  \
+  MI355_KERNEL(256) void mi355_pages_move_l##L##_s##S(mi355::PageMoveArgs a) {        \
+    mi355::page_move_body<L != 0, S>(a);                                              \
+  }
+MI355_FOR_EACH_PAGE_MOVE_KERNEL(MI355_DEFINE_PAGE_MOVE)
+
+MI355_KERNEL(1024) void mi355_pages_reserve(mi355::PageReserveArgs a) { mi355::page_reserve_body(a); }
+MI355_KERNEL(256) void mi355_pages_fork(mi355::PageForkArgs a) { mi355::page_fork_body(a); }
+MI355_KERNEL(256) void mi355_pages_free(mi355::PageFreeArgs a) { mi355::page_free_body(a); }
+MI355_KERNEL(1024) void mi355_pages_compact_plan(mi355::PageCompactArgs a) { mi355::page_compact_plan_body(a); }
+MI355_KERNEL(256) void mi355_pages_compact_apply(mi355::PageCompactArgs a) { mi355::page_compact_apply_body(a); }
+MI355_KERNEL(256) void mi355_pages_compact_tables(mi355::PageCompactArgs a) { mi355::page_compact_tables_body(a); }
+MI355_KERNEL(256) void mi355_pages_reset(mi355::PageResetArgs a) { mi355::page_reset_body(a); }
+
+#endif  // MI355_BLIT_PAGES_KERNELS_H_
