@@ -421,13 +421,13 @@ typedef struct {
 int mi355_blit_pages_book(uint32_t num_pages, uint32_t max_seqs, uint32_t max_pages_per_seq, mi355_blit_book_t* out);
 
 /* A pool, or a pool and its book, on the handle's GPU.  Allocates the work
- * memory of the calls (12 bytes for each page, 32 for each 4 KiB of a page
+ * memory of the calls (12 bytes for each page, 80 for each KiB of a page
  * over all planes), so it cannot be called while a stream is being captured,
  * and neither can mi355_blit_pages_destroy.  A missing plane or base, zero pages, rows,
  * runs or row_bytes, a pitch below the page's bytes, a book without sequences
  * or the other way round -> INVALID_ARGUMENT.  More than 4096 planes, a page of
  * more than 2^31-1 bytes in one plane, sequences of more than 2^31-1 tokens,
- * 2^32 pieces of 4 KiB or more in the pool, or more than the limits above -> OUT_OF_RESOURCES.
+ * 2^32 pieces of 1 KiB or more in the pool, or more than the limits above -> OUT_OF_RESOURCES.
  * The planes' and the book's memory stay the caller's and have to outlive the
  * object, and the object has to be destroyed before the handle. */
 int mi355_blit_pages_create(mi355_blit_t* h, const mi355_blit_pages_desc_t* desc, mi355_blit_pages_t** out);
@@ -450,7 +450,7 @@ int mi355_blit_pages_reset(mi355_blit_pages_t* p, void* stream);
  * Lists that name a page as a destination twice, or both as a source and as a destination,
  * leave the bytes of that page undefined, as overlapping copies do.  NULL
  * list with n > 0, pools that differ -> INVALID_ARGUMENT; n pages of 2^32
- * pieces of 4 KiB or more -> OUT_OF_RESOURCES; n == 0 -> SUCCESS without a launch.
+ * pieces of 1 KiB or more -> OUT_OF_RESOURCES; n == 0 -> SUCCESS without a launch.
  * No book is read or written. */
 int mi355_blit_pages_copy(mi355_blit_pages_t* dst, const int32_t* dst_pages, mi355_blit_pages_t* src,
                           const int32_t* src_pages, const int32_t* valid_rows, size_t n, uint32_t route,

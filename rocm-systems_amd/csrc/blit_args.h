@@ -23,7 +23,7 @@ constexpr unsigned kWave = 64;
 // magic_divisor(d) = ceil(2^64 / d), n / d == (n * m) >> 64 for all n < 2^32
 // (the error n * (m * d - 2^64) stays below 2^64).  d == 1 has no such m in 64
 // bits and is encoded as 0.
-inline uint64_t magic_divisor(uint32_t d) { return d > 1 ? ~0ull / d + 1 : 0; }
+MI355_HOST_DEVICE inline uint64_t magic_divisor(uint32_t d) { return d > 1 ? ~0ull / d + 1 : 0; }
 
 MI355_HOST_DEVICE inline uint32_t div_magic(uint32_t n, uint64_t magic) {
 #ifdef __HIP_DEVICE_COMPILE__

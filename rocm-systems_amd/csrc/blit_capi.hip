@@ -858,10 +858,11 @@ int mi355_blit_plan_rect_route(const mi355_pitched_ptr_t* dst, const mi355_dim3_
 
 struct mi355_blit_pages {
   mi355_blit* h = nullptr;
-  uint32_t num_pages = 0, rows = 0, n_planes = 0, segs = 0;
+  uint32_t num_pages = 0, rows = 0, n_planes = 0;
+  uint32_t pieces[2] = {0, 0};               // of a page, for each size of piece
   uint64_t page_bytes = 0;                  // over all planes
   uint64_t (*planes)[2] = nullptr;          // row_bytes and runs of each, to compare two pools by
-  mi355::PageSegment* segs_dev = nullptr;
+  mi355::PagePlane* planes_dev[2] = {nullptr, nullptr};  // one allocation
   void* work_dev = nullptr;
   bool has_book = false;
   uint64_t book_words = 0;
@@ -872,21 +873,23 @@ struct mi355_blit_pages {
 namespace {
 
 typedef void (*page_move_kernel_t)(PageMoveArgs);
-struct PageMoveVariant { unsigned nt_load, store; page_move_kernel_t fn; };
-#define MI355_PAGE_MOVE_ROW(L, S) {L, S, mi355_pages_move_l##L##_s##S},
+struct PageMoveVariant { unsigned unroll, nt_load, store; page_move_kernel_t fn; };
+#define MI355_PAGE_MOVE_ROW(U, L, S) {U, L, S, mi355_pages_move_u##U##_l##L##_s##S},
 const PageMoveVariant kPageMoveVariants[] = {MI355_FOR_EACH_PAGE_MOVE_KERNEL(MI355_PAGE_MOVE_ROW)};
 
 // n moves, or the first *count of a list with room for n.
 int launch_page_moves(const mi355_blit_pages& to, const mi355_blit_pages& from, const int32_t* dst, const int32_t* src,
-                      const int32_t* valid, const uint32_t* count, uint64_t n, uint32_t route, hipStream_t s) {
-  const PageMovePlan p = plan_page_moves(n, to.segs, to.page_bytes, to.h->num_cus, route, kHostLinkMaxGrid);
+                      const int32_t* valid, const PageMoveCount* count, uint64_t n, uint32_t route, hipStream_t s) {
+  const PageMovePlan p = plan_page_moves(n, count != nullptr, valid != nullptr, to.pieces, to.page_bytes, to.h->num_cus,
+                                         route, kHostLinkMaxGrid);
   page_move_kernel_t k = nullptr;
   for (const PageMoveVariant& v : kPageMoveVariants)
-    if (v.nt_load == p.nt_load && v.store == p.store_policy) k = v.fn;
+    if (v.unroll == kPieceUnrolls[p.table] && v.nt_load == p.nt_load && v.store == p.store_policy) k = v.fn;
   if (!k) return MI355_BLIT_ERROR;
-  const PageMoveArgs a{to.segs_dev, from.segs_dev, dst, src, valid, count, static_cast<uint32_t>(n), to.segs,
-                       magic_divisor(to.segs), to.num_pages, from.num_pages, to.rows, kMoveWaves, p.grid * kMoveWaves, 0};
-  hipLaunchKernelGGL(k, dim3(p.grid), dim3(p.wg_size), 0, s, a);
+  const PageMoveArgs a{to.planes_dev[p.table], from.planes_dev[p.table], dst, src, valid, count,
+                       magic_divisor(static_cast<uint32_t>(n)), static_cast<uint32_t>(n), to.pieces[p.table],
+                       to.num_pages, from.num_pages, to.rows, p.grid * kMoveWaves};
+  hipLaunchKernelGGL(k, dim3(p.grid), dim3(kMoveWaves * kWave), 0, s, a);
   BLIT_HIP(hipGetLastError());
   return MI355_BLIT_SUCCESS;
 }
@@ -908,14 +911,14 @@ int mi355_blit_pages_create(mi355_blit_t* h, const mi355_blit_pages_desc_t* desc
   if (!out) return MI355_BLIT_ERROR_INVALID_ARGUMENT;
   *out = nullptr;
   if (!h) return MI355_BLIT_ERROR_INVALID_ARGUMENT;
-  uint64_t segs = 0;
-  int rc = pages_check(desc, &segs);
+  uint64_t pieces = 0;
+  int rc = pages_check(desc, &pieces);
   if (rc != MI355_BLIT_SUCCESS) return rc;
   std::lock_guard<std::mutex> g(h->lock);
   DeviceScope scope(h->device);
   if (scope.err != hipSuccess) return status_of(scope.err);
   mi355_blit_pages* p = new (std::nothrow) mi355_blit_pages;
-  PageSegment* table = static_cast<PageSegment*>(std::malloc(segs * sizeof(PageSegment)));
+  PagePlane* table = static_cast<PagePlane*>(std::malloc(2 * pieces * sizeof(PagePlane)));
   if (p) p->planes = static_cast<uint64_t(*)[2]>(std::malloc(desc->n_planes * sizeof(*p->planes)));
   hipError_t e = p && table && p->planes ? hipSuccess : hipErrorOutOfMemory;
   if (e == hipSuccess) {
@@ -923,17 +926,20 @@ int mi355_blit_pages_create(mi355_blit_t* h, const mi355_blit_pages_desc_t* desc
     p->num_pages = desc->num_pages;
     p->rows = desc->rows;
     p->n_planes = desc->n_planes;
-    p->segs = static_cast<uint32_t>(segs);
     for (uint32_t i = 0; i < desc->n_planes; ++i) {
       p->planes[i][0] = desc->planes[i].row_bytes;
       p->planes[i][1] = desc->planes[i].runs;
       p->page_bytes += plane_page_bytes(desc->planes[i], desc->rows);
     }
-    pages_segments(*desc, table);
-    e = hipMalloc(reinterpret_cast<void**>(&p->segs_dev), segs * sizeof(PageSegment));
+    p->pieces[0] = pages_planes(*desc, kPieceUnrolls[0], table);
+    p->pieces[1] = pages_planes(*desc, kPieceUnrolls[1], table + p->pieces[0]);
+    e = hipMalloc(reinterpret_cast<void**>(&p->planes_dev[0]), (p->pieces[0] + p->pieces[1]) * sizeof(PagePlane));
   }
   // through the default stream, and waited for
-  if (e == hipSuccess) e = hipMemcpy(p->segs_dev, table, segs * sizeof(PageSegment), hipMemcpyHostToDevice);
+  if (e == hipSuccess) {
+    p->planes_dev[1] = p->planes_dev[0] + p->pieces[0];
+    e = hipMemcpy(p->planes_dev[0], table, (p->pieces[0] + p->pieces[1]) * sizeof(PagePlane), hipMemcpyHostToDevice);
+  }
   if (e == hipSuccess && desc->max_seqs) {
     mi355_blit_book_t at;
     rc = pages_book_layout(desc->num_pages, desc->max_seqs, desc->max_pages_per_seq, &at);
@@ -946,7 +952,7 @@ int mi355_blit_pages_create(mi355_blit_t* h, const mi355_blit_pages_desc_t* desc
     if (rc == MI355_BLIT_SUCCESS) e = hipMalloc(&p->work_dev, words * sizeof(int32_t));
     if (rc == MI355_BLIT_SUCCESS && e == hipSuccess) {
       int32_t* w = static_cast<int32_t*>(p->work_dev);
-      p->moves = {w + 64, w + 64 + room, w + 64 + 2 * room, w + 64 + 3 * room, reinterpret_cast<uint32_t*>(w)};
+      p->moves = {w + 64, w + 64 + room, w + 64 + 2 * room, w + 64 + 3 * room, reinterpret_cast<PageMoveCount*>(w)};
     }
   }
   std::free(table);
@@ -955,7 +961,7 @@ int mi355_blit_pages_create(mi355_blit_t* h, const mi355_blit_pages_desc_t* desc
     return MI355_BLIT_SUCCESS;
   }
   if (p) {
-    if (p->segs_dev) (void)hipFree(p->segs_dev);
+    if (p->planes_dev[0]) (void)hipFree(p->planes_dev[0]);
     if (p->work_dev) (void)hipFree(p->work_dev);
     std::free(p->planes);
     delete p;
@@ -971,7 +977,7 @@ int mi355_blit_pages_destroy(mi355_blit_pages_t* p) {
     if (scope.err != hipSuccess) return status_of(scope.err);
     // commands may be on any stream; memory that they still use is not freed
     BLIT_HIP(hipDeviceSynchronize());
-    (void)hipFree(p->segs_dev);
+    (void)hipFree(p->planes_dev[0]);
     if (p->work_dev) (void)hipFree(p->work_dev);
   }
   std::free(p->planes);
@@ -1000,7 +1006,7 @@ int mi355_blit_pages_copy(mi355_blit_pages_t* dst, const int32_t* dst_pages, mi3
                      std::memcmp(dst->planes, src->planes, dst->n_planes * sizeof(*dst->planes)) != 0))
     return MI355_BLIT_ERROR_INVALID_ARGUMENT;
   if (n == 0) return MI355_BLIT_SUCCESS;
-  if (n > 0xffffffffull / dst->segs) return MI355_BLIT_ERROR_OUT_OF_RESOURCES;
+  if (n > 0xffffffffull / dst->pieces[0]) return MI355_BLIT_ERROR_OUT_OF_RESOURCES;
   std::lock_guard<std::mutex> g(dst->h->lock);
   DeviceScope scope(dst->h->device);
   if (scope.err != hipSuccess) return status_of(scope.err);

@@ -178,18 +178,29 @@ MI355_DEVICE uint32_t ld_uniform_u32(const uint32_t* p) {
 #pragma clang diagnostic pop
 }
 
-// A segment of a page, at an address that is the same for every lane, through
-// the constant address space like a record.
-MI355_DEVICE PageSegment ld_uniform_segment(const PageSegment* p) {
-  typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
-  typedef const u32x8 __attribute__((address_space(4))) * ConstPtr;
+// A plane of a pool, at an address that is the same for every lane, through the
+// constant address space like a record.
+MI355_DEVICE PagePlane ld_uniform_plane(const PagePlane* p) {
+  typedef uint32_t u32x16 __attribute__((ext_vector_type(16)));
+  typedef const u32x16 __attribute__((address_space(4))) * ConstPtr;
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Wold-style-cast"
-  const u32x8 v = *(ConstPtr)(p);
+  const u32x16 v = *(ConstPtr)(p);
 #pragma clang diagnostic pop
-  PageSegment s;
-  __builtin_memcpy(&s, &v, sizeof(s));
-  return s;
+  PagePlane r;
+  __builtin_memcpy(&r, &v, sizeof(r));
+  return r;
+}
+MI355_DEVICE PageMoveCount ld_uniform_count(const PageMoveCount* p) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  typedef const u32x4 __attribute__((address_space(4))) * ConstPtr;
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Wold-style-cast"
+  const u32x4 v = *(ConstPtr)(p);
+#pragma clang diagnostic pop
+  PageMoveCount r;
+  __builtin_memcpy(&r, &v, sizeof(r));
+  return r;
 }
 
 // Words that other workgroups of the same launch change too: read, and changed

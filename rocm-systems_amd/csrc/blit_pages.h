@@ -1,6 +1,6 @@
 // Pages of a key/value cache: argument blocks of their kernels, and the host
 // arithmetic in front of them (the layout of a book, the check of a pool's
-// geometry, the cut of a page into segments, launch sizes).  Plain C++, no HIP.
+// geometry, the table of its planes, launch sizes).  Plain C++, no HIP.
 //
 // A pool is a set of planes; page q of plane p is at base_p + q * pitch_p and
 // is runs_p runs of `rows` rows of row_bytes_p bytes, one behind the other.  A
@@ -12,47 +12,59 @@
 #include <stdint.h>
 
 #include "blit_args.h"
+#include "blit_plan.h"
 #include "mi355_blit.h"
 
 namespace mi355 {
 
-// 16-byte vectors each lane keeps in flight, and with that the bytes of a page
-// that one wave moves at a time.
-constexpr unsigned kPageUnroll = 4;
-constexpr uint32_t kSegmentBytes = kWave * 16 * kPageUnroll;
+// A wave moves a piece of a page at a time: 16 bytes for each lane, or four
+// times that where the first rows of the pages are moved only, so that fewer
+// waves find nothing to do (190 pages of 24 planes, half of their rows: 13.3 us
+// against 15.8; 600 pages of 1 MiB 134 against 153; whole pages, 800 of 1 MiB:
+// 285 us with 1 KiB, 330 with 4 KiB).
+constexpr unsigned kPieceUnrolls[] = {1, 4};
+constexpr uint32_t piece_bytes(unsigned unroll) { return kWave * 16 * unroll; }
 
-// One wave's share of a page: `bytes` bytes at `offset` of the page of one
-// plane.  The table of all segments of a page, over all planes, is made once
-// for a pool; a wave of a move reads one record from it and needs nothing else
-// than the number of the page.
-struct __attribute__((aligned(32))) PageSegment {
-  uint8_t* base;  // the segment in page 0 (the plane's base + offset)
+// What a wave needs to know of a plane.  The tables of a pool, made once, one for
+// each size of piece, have a record for each piece of a page, counted through all
+// planes, and all records of a plane are the same: work item w of n moves belongs
+// to the plane of piece w / n, whatever n is.
+struct __attribute__((aligned(64))) PagePlane {
+  uint8_t* base;
   uint64_t pitch;
-  uint32_t offset;
-  uint32_t bytes;      // <= kSegmentBytes
-  uint32_t run_bytes;  // rows * row_bytes; 0 where the page is one run
+  uint64_t magic_pieces;  // magic_divisor(pieces)
+  uint32_t pieces;        // of a page in this plane
+  uint32_t first;         // pieces of the planes before it
+  uint32_t bytes;         // of a page in this plane
+  uint32_t run_bytes;     // rows * row_bytes; 0 where the page is one run
   uint32_t row_bytes;
+  uint32_t pad[3];
 };
-static_assert(sizeof(PageSegment) == 32, "one s_load_dwordx8");
+static_assert(sizeof(PagePlane) == 64, "one s_load_dwordx16");
 
-// Pages src[i] to pages dst[i], in all planes: work item w is segment w % segs
-// of move w / segs.
+// The number of moves that a call has decided on the device, with what it takes
+// to divide by it.
+struct PageMoveCount {
+  uint32_t n;
+  uint32_t pad;
+  uint64_t magic;  // magic_divisor(n)
+};
+
+// Pages src[i] to pages dst[i], in all planes.
 struct PageMoveArgs {
-  const PageSegment* dst_segs;
-  const PageSegment* src_segs;
+  const PagePlane* dst_planes;
+  const PagePlane* src_planes;
   const int32_t* dst;
   const int32_t* src;
-  const int32_t* valid;   // rows of every run that are moved; null: all
-  const uint32_t* count;  // the number of moves, at most n; null: n
+  const int32_t* valid;        // rows of every run that are moved; null: all
+  const PageMoveCount* count;  // the number of moves, at most n; null: n
+  uint64_t magic_n;            // magic_divisor(n)
   uint32_t n;
-  uint32_t segs;
-  uint64_t magic_segs;  // magic_divisor(segs)
-  uint32_t dst_pages;   // pages of each pool: others are not moved
+  uint32_t pieces;     // of a page, over all planes
+  uint32_t dst_pages;  // pages of each pool: others are not moved
   uint32_t src_pages;
   uint32_t rows;
-  uint32_t waves_per_wg;
   uint32_t n_waves;
-  uint32_t pad;
 };
 
 // The parts of a book on the device.
@@ -75,7 +87,7 @@ struct PageMoveList {
   int32_t* dst;
   int32_t* valid;   // reserve only
   int32_t* remap;   // compact only: the new number of a page that moved
-  uint32_t* count;
+  PageMoveCount* count;
 };
 
 struct PageReserveArgs {
@@ -153,8 +165,8 @@ inline uint64_t plane_page_bytes(const mi355_blit_plane_t& p, uint32_t rows) {
   return run * p.runs;
 }
 
-// What mi355_blit_pages_create takes; *segs gets the number of segments of a page.
-inline int pages_check(const mi355_blit_pages_desc_t* d, uint64_t* segs) {
+// What mi355_blit_pages_create takes; *pieces gets the number of the smallest pieces of a page.
+inline int pages_check(const mi355_blit_pages_desc_t* d, uint64_t* pieces) {
   if (!d || !d->planes || d->n_planes == 0 || d->num_pages == 0 || d->rows == 0) return MI355_BLIT_ERROR_INVALID_ARGUMENT;
   if ((d->max_seqs == 0) != (d->book == nullptr) || (d->max_seqs == 0) != (d->max_pages_per_seq == 0))
     return MI355_BLIT_ERROR_INVALID_ARGUMENT;
@@ -173,51 +185,73 @@ inline int pages_check(const mi355_blit_pages_desc_t* d, uint64_t* segs) {
     const unsigned __int128 end = static_cast<unsigned __int128>(d->num_pages - 1) * p.pitch + page +
                                   reinterpret_cast<uintptr_t>(p.base);
     if (end >> 64) return MI355_BLIT_ERROR_INVALID_ARGUMENT;
-    total += (page + kSegmentBytes - 1) / kSegmentBytes;
+    total += (page + piece_bytes(1) - 1) / piece_bytes(1);
   }
   // work items are counted in 32 bits
   if (total * d->num_pages > 0xffffffffull) return MI355_BLIT_ERROR_OUT_OF_RESOURCES;
-  *segs = total;
+  *pieces = total;
   return MI355_BLIT_SUCCESS;
 }
 
-// The segments of a page, plane by plane; `out` has room for what pages_check counted.
-inline void pages_segments(const mi355_blit_pages_desc_t& d, PageSegment* out) {
+// The table of a pool for one size of piece; returns the number of its records.
+// `out` may be null, and has room for what pages_check counted otherwise.
+inline uint32_t pages_planes(const mi355_blit_pages_desc_t& d, unsigned unroll, PagePlane* out) {
+  uint32_t first = 0;
   for (uint32_t i = 0; i < d.n_planes; ++i) {
     const mi355_blit_plane_t& p = d.planes[i];
-    const uint32_t page = static_cast<uint32_t>(plane_page_bytes(p, d.rows));
-    for (uint32_t at = 0; at < page; at += kSegmentBytes) {
-      PageSegment s;
-      s.base = static_cast<uint8_t*>(p.base) + at;
-      s.pitch = p.pitch;
-      s.offset = at;
-      s.bytes = page - at < kSegmentBytes ? page - at : kSegmentBytes;
-      s.run_bytes = p.runs > 1 ? d.rows * p.row_bytes : 0;
-      s.row_bytes = p.row_bytes;
-      *out++ = s;
-    }
+    PagePlane r{};
+    r.base = static_cast<uint8_t*>(p.base);
+    r.pitch = p.pitch;
+    r.bytes = static_cast<uint32_t>(plane_page_bytes(p, d.rows));
+    r.pieces = (r.bytes + piece_bytes(unroll) - 1) / piece_bytes(unroll);
+    r.magic_pieces = magic_divisor(r.pieces);
+    r.first = first;
+    r.run_bytes = p.runs > 1 ? d.rows * p.row_bytes : 0;
+    r.row_bytes = p.row_bytes;
+    for (uint32_t k = 0; out && k < r.pieces; ++k) out[first + k] = r;
+    first += r.pieces;
   }
+  return first;
 }
 
 struct PageMovePlan {
-  uint32_t nt_load, store_policy, wg_size, grid;
+  uint32_t table;  // index into kPieceUnrolls
+  uint32_t nt_load, store_policy, grid;
 };
 
-// A wave for every segment, up to a grid that fills the device: the list of a
-// call that decides its moves on the device is as long as it could be, and
-// mostly empty.  Over the host link at most kLinkGrid workgroups, as for the
-// linear copy; what goes to the host is written through at once.
+// How n moves are launched; `listed`: n is what the list has room for, the
+// device knows how many there are.  pieces: of a page, for each size of piece.
+//
+// Cache policy, by the bytes that are likely moved (half of the pages where only
+// their first rows are).  Measured, pages of 32 planes of 32 KiB, loads and stores cached /
+// non-temporal loads with stores written through / with non-temporal stores:
+// 64 MiB 22.8 / 22.0 / 27.7 us, 128 MiB 42.9 / 41.9 / 51.0, 192 MiB 79.2 / 61.0 /
+// 74.2, 256 MiB 106.7 / 83.1 / 98.5, 384 MiB 156 / 153 / 143, 600 MiB 237 / 239 / 221.
+//
+// A wave for each piece: the dispatcher hands pieces out in order, which keeps
+// what is in flight close together (1 GiB, 32 KiB a page and plane: 369 us; a
+// grid of 8 workgroups for each CU whose waves stride 446, and 425 with the next piece's loads
+// in front of the stores).  A list of unknown length is as long as its room: a
+// wave too many costs 0.05 ns, so kMostListed workgroups for each CU (26 us of them
+// at most), and strides beyond (800 MiB 292 us; with 128 for each CU 325).
+// Over the host link at most link_grid workgroups, as for the linear copy; what
+// goes to the host is written through at once.
 constexpr uint32_t kMoveWaves = 4;
-inline PageMovePlan plan_page_moves(uint64_t n, uint64_t segs, uint64_t page_bytes, uint32_t num_cus, uint32_t route,
-                                    uint32_t link_grid) {
+constexpr uint32_t kMostListed = 512;
+constexpr uint64_t kMoveStreams = 128ull << 20, kMoveNtStores = 320ull << 20;
+
+inline PageMovePlan plan_page_moves(uint64_t n, bool listed, bool cut, const uint32_t (&pieces)[2], uint64_t page_bytes,
+                                    uint32_t num_cus, uint32_t route, uint32_t link_grid) {
   PageMovePlan p;
-  const bool large = n * page_bytes >= (4ull << 20);
-  p.nt_load = large;
+  p.table = cut ? 1 : 0;
+  const uint64_t bytes = cut ? n * page_bytes / 2 : n * page_bytes;
+  p.nt_load = bytes >= kMoveStreams;
   p.store_policy = route == MI355_BLIT_ROUTE_DEVICE_TO_HOST ? MI355_BLIT_STORE_SYSTEM_WT
-                   : large ? MI355_BLIT_STORE_AGENT_WT : MI355_BLIT_STORE_CACHED;
-  p.wg_size = kMoveWaves * kWave;
-  const uint64_t want = (n * segs + kMoveWaves - 1) / kMoveWaves;
-  const uint64_t most = route == MI355_BLIT_ROUTE_DEVICE ? static_cast<uint64_t>(num_cus) * 8 : link_grid;
+                   : bytes >= kMoveNtStores ? MI355_BLIT_STORE_NT
+                   : bytes >= kMoveStreams ? MI355_BLIT_STORE_AGENT_WT : MI355_BLIT_STORE_CACHED;
+  const uint64_t want = (n * pieces[p.table] + kMoveWaves - 1) / kMoveWaves;
+  const uint64_t most = route != MI355_BLIT_ROUTE_DEVICE ? link_grid
+                        : listed ? static_cast<uint64_t>(num_cus) * kMostListed : kMaxGridWorkItems / (kMoveWaves * kWave);
   p.grid = static_cast<uint32_t>(want < most ? want : most);
   return p;
 }

@@ -15,68 +15,75 @@
 namespace mi355 {
 
 // ---------------------------------------------------------------------------
-// Moves.  One wave moves one segment (4 KiB: four 16-byte loads of each lane
-// in flight before the first store).  Bound by memory: 2 bytes of traffic for
-// each byte of the pages that are named, nothing else.
+// Moves.  One wave moves one piece of a page.  Work items go through the
+// planes one after the other, in each through the moves, and in each move through
+// the pieces of the page.  Bound by memory: 2 bytes of traffic for each byte of
+// the pages that are named, nothing else.
 // ---------------------------------------------------------------------------
 
 // A page of several runs of which only the first rows are moved: the bytes
 // whose place in their run is below `limit`.  A vector may lie across the end
-// of the rows or of a run; such a one goes byte by byte.
+// of the rows or of a run; such a one goes byte by byte.  `offset` is the
+// piece's place in the page, `bytes` its length.
 template <bool NTL, int ST>
-MI355_DEVICE void move_cut_runs(uint8_t* d, const uint8_t* s, const PageSegment& g, unsigned limit, unsigned lane) {
-  for (unsigned at = 16 * lane; at < g.bytes; at += 16 * kWave) {
-    const unsigned in_run = (g.offset + at) % g.run_bytes;
-    const unsigned left = g.bytes - at;
+MI355_DEVICE void move_cut_runs(uint8_t* d, const uint8_t* s, const PagePlane& g, unsigned offset, unsigned bytes,
+                                unsigned limit, unsigned lane) {
+  for (unsigned at = 16 * lane; at < bytes; at += 16 * kWave) {
+    const unsigned in_run = (offset + at) % g.run_bytes;
+    const unsigned left = bytes - at;
     if (left >= 16 && in_run + 16 <= limit) {
       st_v4_any<ST>(reinterpret_cast<uintptr_t>(d + at), ld_v4_any<NTL>(s + at));
     } else if (in_run < limit || in_run + 16 > g.run_bytes) {
       const unsigned n = left < 16 ? left : 16;
       for (unsigned b = 0; b < n; ++b)
-        if ((g.offset + at + b) % g.run_bytes < limit) st_u8(d + at + b, ld_u8(s + at + b));
+        if ((offset + at + b) % g.run_bytes < limit) st_u8(d + at + b, ld_u8(s + at + b));
     }
   }
 }
 
-template <bool NTL, int ST>
-MI355_DEVICE void move_segment(uint8_t* d, const uint8_t* s, const PageSegment& g, unsigned valid, unsigned rows,
-                               unsigned lane) {
-  unsigned bytes = g.bytes;
+template <int U, bool NTL, int ST>
+MI355_DEVICE void move_piece(uint8_t* d, const uint8_t* s, const PagePlane& g, unsigned offset, unsigned valid,
+                             unsigned rows, unsigned lane) {
+  unsigned bytes = g.bytes - offset < piece_bytes(U) ? g.bytes - offset : piece_bytes(U);
   if (valid < rows) {
     const unsigned limit = valid * g.row_bytes;
     if (g.run_bytes) {
-      move_cut_runs<NTL, ST>(d, s, g, limit, lane);
+      move_cut_runs<NTL, ST>(d, s, g, offset, bytes, limit, lane);
       return;
     }
-    if (limit <= g.offset) return;
-    if (limit - g.offset < bytes) bytes = limit - g.offset;
+    if (limit <= offset) return;
+    if (limit - offset < bytes) bytes = limit - offset;
   }
   const unsigned vecs = bytes / 16;
-  v4u x[kPageUnroll];
+  v4u x[U];
 #pragma unroll
-  for (unsigned u = 0; u < kPageUnroll; ++u)
+  for (unsigned u = 0; u < U; ++u)
     if (lane + u * kWave < vecs) x[u] = ld_v4_any<NTL>(s + 16 * (lane + u * kWave));
 #pragma unroll
-  for (unsigned u = 0; u < kPageUnroll; ++u)
+  for (unsigned u = 0; u < U; ++u)
     if (lane + u * kWave < vecs) st_v4_any<ST>(reinterpret_cast<uintptr_t>(d + 16 * (lane + u * kWave)), x[u]);
   const unsigned tail = bytes & 15;
   if (lane < tail) st_u8(d + 16 * vecs + lane, ld_u8(s + 16 * vecs + lane));
 }
 
-template <bool NTL, int ST>
+template <int U, bool NTL, int ST>
 MI355_DEVICE void page_move_body(const PageMoveArgs& a) {
   const unsigned lane = thread_in_workgroup() & (kWave - 1);
   uint32_t n = a.n;
+  uint64_t magic_n = a.magic_n;
   if (a.count) {
-    const uint32_t found = ld_uniform_u32(a.count);
-    if (found < n) n = found;
+    const PageMoveCount found = ld_uniform_count(a.count);
+    if (found.n < n) n = found.n, magic_n = found.magic;
   }
-  // n * segs fits in 32 bits, and so does what a wave adds to get past it
-  // (checked on the host): 64 bits only for the sum
-  const uint64_t total = static_cast<uint64_t>(n) * a.segs;
-  for (uint64_t w = global_wave(a.waves_per_wg); w < total; w += a.n_waves) {
-    const uint32_t move = div_magic(static_cast<uint32_t>(w), a.magic_segs);
-    const uint32_t seg = static_cast<uint32_t>(w) - move * a.segs;
+  // fits in 32 bits (checked on the host); the sum with n_waves may not
+  const uint64_t total = static_cast<uint64_t>(n) * a.pieces;
+  for (uint64_t w = global_wave(kMoveWaves); w < total; w += a.n_waves) {
+    const uint32_t item = static_cast<uint32_t>(w);
+    const uint32_t some_piece = div_magic(item, magic_n);
+    const PagePlane d = ld_uniform_plane(a.dst_planes + some_piece);
+    const uint32_t in_plane = item - n * d.first;
+    const uint32_t move = div_magic(in_plane, d.magic_pieces);
+    const uint32_t offset = (in_plane - move * d.pieces) * piece_bytes(U);
     const uint32_t to = ld_uniform_u32(reinterpret_cast<const uint32_t*>(a.dst + move));
     const uint32_t from = ld_uniform_u32(reinterpret_cast<const uint32_t*>(a.src + move));
     uint32_t valid = a.rows;
@@ -86,9 +93,8 @@ MI355_DEVICE void page_move_body(const PageMoveArgs& a) {
     }
     // a negative number is a large unsigned one
     if (to >= a.dst_pages || from >= a.src_pages || valid == 0) continue;
-    const PageSegment d = ld_uniform_segment(a.dst_segs + seg);
-    const PageSegment s = ld_uniform_segment(a.src_segs + seg);
-    move_segment<NTL, ST>(d.base + to * d.pitch, s.base + from * s.pitch, s, valid, a.rows, lane);
+    const PagePlane s = ld_uniform_plane(a.src_planes + some_piece);
+    move_piece<U, NTL, ST>(d.base + to * d.pitch + offset, s.base + from * s.pitch + offset, d, offset, valid, a.rows, lane);
   }
 }
 
@@ -316,7 +322,7 @@ MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
     wait_for_memory();
     workgroup_barrier();
   }
-  if (t == 0) st_obj(a.moves.count, n_moves);
+  if (t == 0) st_obj(a.moves.count, PageMoveCount{n_moves, 0, magic_divisor(n_moves)});
 }
 
 // A sequence that holds its parent's pages.  A workgroup of 256 lanes for each
@@ -439,7 +445,7 @@ MI355_DEVICE void page_compact_plan_body(const PageCompactArgs& a) {
   }
   if (t == 0) {
     const uint32_t n = holes < a.max_moves ? holes : a.max_moves;
-    st_obj(a.moves.count, n);
+    st_obj(a.moves.count, PageMoveCount{n, 0, magic_divisor(n)});
     st_obj(b.head, static_cast<int32_t>(n));
   }
 }
@@ -447,7 +453,7 @@ MI355_DEVICE void page_compact_plan_body(const PageCompactArgs& a) {
 // The counts and free bits of the pages that move, a lane for each.
 MI355_DEVICE void page_compact_apply_body(const PageCompactArgs& a) {
   const BookPtrs& b = a.book;
-  const uint32_t n = ld_uniform_u32(a.moves.count);
+  const uint32_t n = ld_uniform_u32(&a.moves.count->n);
   const uint32_t k = workgroup_index() * 256 + thread_in_workgroup();
   if (k >= n) return;
   const uint32_t from = ld_obj(a.moves.src + k), to = ld_obj(a.moves.dst + k);
@@ -466,7 +472,7 @@ MI355_DEVICE void page_compact_apply_body(const PageCompactArgs& a) {
 // are the highest ones, so every held page from the lowest of them on has moved.
 MI355_DEVICE void page_compact_tables_body(const PageCompactArgs& a) {
   const BookPtrs& b = a.book;
-  const uint32_t n = ld_uniform_u32(a.moves.count);
+  const uint32_t n = ld_uniform_u32(&a.moves.count->n);
   if (n == 0) return;
   const uint32_t lowest = ld_uniform_u32(reinterpret_cast<const uint32_t*>(a.moves.src + n - 1));
   const uint32_t s = workgroup_index();
@@ -499,11 +505,12 @@ MI355_DEVICE void page_reset_body(const PageResetArgs& a) {
 }  // namespace mi355
 
 // Entry points, named as those of blit_kernels.h:
-//   mi355_pages_move_l<nt loads>_s<store policy>
-#define MI355_FOR_EACH_PAGE_MOVE_KERNEL(X) X(0, 0) X(1, 2) X(0, 3) X(1, 3)
-#define MI355_DEFINE_PAGE_MOVE(L, S)                                                  \
-  MI355_KERNEL(256) void mi355_pages_move_l##L##_s##S(mi355::PageMoveArgs a) {        \
-    mi355::page_move_body<L != 0, S>(a);                                              \
+//   mi355_pages_move_u<16-byte vectors a lane>_l<nt loads>_s<store policy>
+#define MI355_PAGE_MOVE_LS_(X, U) X(U, 0, 0) X(U, 1, 1) X(U, 1, 2) X(U, 0, 3) X(U, 1, 3)
+#define MI355_FOR_EACH_PAGE_MOVE_KERNEL(X) MI355_PAGE_MOVE_LS_(X, 1) MI355_PAGE_MOVE_LS_(X, 4)
+#define MI355_DEFINE_PAGE_MOVE(U, L, S)                                                       \
+  MI355_KERNEL(256) void mi355_pages_move_u##U##_l##L##_s##S(mi355::PageMoveArgs a) {         \
+    mi355::page_move_body<U, L != 0, S>(a);                                                   \
   }
 MI355_FOR_EACH_PAGE_MOVE_KERNEL(MI355_DEFINE_PAGE_MOVE)
 

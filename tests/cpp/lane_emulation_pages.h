@@ -1,5 +1,5 @@
-// lane_emulation.h with what the page kernels use beyond it: scalar segment
-// loads, atomics on memory and on LDS, bit counts, and workgroups that run in
+// lane_emulation.h with what the page kernels use beyond it: scalar loads
+// of their records, atomics on memory and on LDS, bit counts, and workgroups that run in
 // the reverse order on request (the result of a launch may not depend on it).
 #ifndef MI355_TESTS_LANE_EMULATION_PAGES_H_
 #define MI355_TESTS_LANE_EMULATION_PAGES_H_
@@ -17,7 +17,8 @@ MI355_DEVICE unsigned workgroup_index() {
   return g_reverse_grid ? g_reverse_grid - 1 - launch_order_index() : launch_order_index();
 }
 
-MI355_DEVICE PageSegment ld_uniform_segment(const PageSegment* p) { return lane_emu::checked_load<PageSegment>(p, 32); }
+MI355_DEVICE PagePlane ld_uniform_plane(const PagePlane* p) { return lane_emu::checked_load<PagePlane>(p, 64); }
+MI355_DEVICE PageMoveCount ld_uniform_count(const PageMoveCount* p) { return lane_emu::checked_load<PageMoveCount>(p, 8); }
 
 // A lane runs until its next lane move or barrier, so these are atomic.
 template <typename T, typename F>

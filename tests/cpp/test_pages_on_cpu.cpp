@@ -60,16 +60,17 @@ struct Bytes {
   }
 };
 
-// A pool with the product's segment table, and the same bytes once more.
+// A pool with the product's table, and the same bytes once more.
 struct Pool {
   Config c;
   std::vector<Bytes> mem;
   std::vector<std::vector<uint8_t>> want;
-  PageSegment* segs = nullptr;
-  uint64_t n_segs = 0, page_bytes = 0;
+  PagePlane* table[2] = {nullptr, nullptr};
+  uint32_t pieces[2] = {0, 0};
+  uint64_t page_bytes = 0;
   Pool() {}
   Pool(const Pool&) = delete;
-  ~Pool() { std::free(segs); }
+  ~Pool() { std::free(table[0]), std::free(table[1]); }
   bool make(const Config& config, bool fresh_pitch) {
     c = config;
     mem.resize(c.planes.size());
@@ -83,11 +84,16 @@ struct Pool {
       page_bytes += page;
     }
     mi355_blit_pages_desc_t d = desc(nullptr);
-    if (pages_check(&d, &n_segs) != MI355_BLIT_SUCCESS) return false;
-    void* q = nullptr;
-    if (posix_memalign(&q, 32, n_segs * sizeof(PageSegment))) std::abort();
-    segs = static_cast<PageSegment*>(q);
-    pages_segments(d, segs);
+    uint64_t counted = 0;
+    if (pages_check(&d, &counted) != MI355_BLIT_SUCCESS) return false;
+    for (int k = 0; k < 2; ++k) {
+      pieces[k] = pages_planes(d, kPieceUnrolls[k], nullptr);
+      if (pieces[k] > counted) return false;
+      void* q = nullptr;
+      if (posix_memalign(&q, 64, pieces[k] * sizeof(PagePlane))) std::abort();
+      table[k] = static_cast<PagePlane*>(q);
+      pages_planes(d, kPieceUnrolls[k], table[k]);
+    }
     return true;
   }
   mi355_blit_pages_desc_t desc(int32_t* book) const {
@@ -99,7 +105,7 @@ struct Pool {
       g_check.allow_read(m.p, m.n);
       if (write) g_check.allow_write(m.p, m.n);
     }
-    g_check.allow_read(segs, n_segs * sizeof(PageSegment));
+    for (int k = 0; k < 2; ++k) g_check.allow_read(table[k], pieces[k] * sizeof(PagePlane));
   }
   // what a copy of the first `valid` rows of page `from` of pool `src` leaves
   void move(const Pool& src, uint32_t from, uint32_t to, uint32_t valid, const std::vector<std::vector<uint8_t>>& before) {
@@ -153,7 +159,7 @@ struct Cache {
     room = c.pages > 2 * kMaxList ? c.pages / 2 : kMaxList;
     work.assign(64 + 3 * room + c.pages, 0x55555555);
     int32_t* w = work.data();
-    moves = {w + 64, w + 64 + room, w + 64 + 2 * room, w + 64 + 3 * room, reinterpret_cast<uint32_t*>(w)};
+    moves = {w + 64, w + 64 + room, w + 64 + 2 * room, w + 64 + 3 * room, reinterpret_cast<PageMoveCount*>(w)};
     start();
     run(mi355_pages_reset, PageResetArgs{ptrs, at.words}, static_cast<uint32_t>((at.words + 255) / 256), 256);
     lengths.assign(c.seqs, 0);
@@ -188,12 +194,18 @@ struct Cache {
   }
 
   static void run_moves(const Pool& to, const Pool& from, const int32_t* dst, const int32_t* src, const int32_t* valid,
-                        const uint32_t* count, uint64_t n, uint32_t route, uint32_t cus) {
-    const PageMovePlan p = plan_page_moves(n, to.n_segs, to.page_bytes, cus, route, 3);
-    const PageMoveArgs a{to.segs, from.segs, dst, src, valid, count, static_cast<uint32_t>(n),
-                         static_cast<uint32_t>(to.n_segs), magic_divisor(static_cast<uint32_t>(to.n_segs)), to.c.pages,
-                         from.c.pages, to.c.rows, kMoveWaves, p.grid * kMoveWaves, 0};
-#define TRY(L, S) if (p.nt_load == L && p.store_policy == S) return run(mi355_pages_move_l##L##_s##S, a, p.grid, p.wg_size);
+                        const PageMoveCount* count, uint64_t n, uint32_t route, uint32_t cus) {
+    PageMovePlan p = plan_page_moves(n, count != nullptr, valid != nullptr, to.pieces, to.page_bytes, cus, route, 3);
+    // the sizes here are small: the policies of large moves, and grids that stride
+    if (p.store_policy == MI355_BLIT_STORE_CACHED && below(2)) p.nt_load = 1, p.store_policy = 1 + below(2);
+    if (p.store_policy == MI355_BLIT_STORE_SYSTEM_WT) p.nt_load = below(2);
+    if (below(2) && p.grid > 3) p.grid = 1 + below(p.grid);
+    const PageMoveArgs a{to.table[p.table], from.table[p.table], dst, src, valid, count,
+                         magic_divisor(static_cast<uint32_t>(n)), static_cast<uint32_t>(n), to.pieces[p.table],
+                         to.c.pages, from.c.pages, to.c.rows, p.grid * kMoveWaves};
+#define TRY(U, L, S) \
+  if (kPieceUnrolls[p.table] == U && p.nt_load == L && p.store_policy == S) \
+    return run(mi355_pages_move_u##U##_l##L##_s##S, a, p.grid, kMoveWaves * kWave);
     MI355_FOR_EACH_PAGE_MOVE_KERNEL(TRY)
 #undef TRY
     fail("no kernel for the plan");
