@@ -421,7 +421,7 @@ typedef struct {
 int mi355_blit_pages_book(uint32_t num_pages, uint32_t max_seqs, uint32_t max_pages_per_seq, mi355_blit_book_t* out);
 
 /* A pool, or a pool and its book, on the handle's GPU.  Allocates the work
- * memory of the calls (12 bytes for each page, 80 for each KiB of a page
+ * memory of the calls (8 bytes for each page, 80 for each KiB of a page
  * over all planes), so it cannot be called while a stream is being captured,
  * and neither can mi355_blit_pages_destroy.  A missing plane or base, zero pages, rows,
  * runs or row_bytes, a pitch below the page's bytes, a book without sequences

@@ -868,6 +868,7 @@ struct mi355_blit_pages {
   uint64_t book_words = 0;
   mi355::BookPtrs book{};
   mi355::PageMoveList moves{};
+  mi355::PageReserveWork reserve{};
 };
 
 namespace {
@@ -876,20 +877,30 @@ typedef void (*page_move_kernel_t)(PageMoveArgs);
 struct PageMoveVariant { unsigned unroll, nt_load, store; page_move_kernel_t fn; };
 #define MI355_PAGE_MOVE_ROW(U, L, S) {U, L, S, mi355_pages_move_u##U##_l##L##_s##S},
 const PageMoveVariant kPageMoveVariants[] = {MI355_FOR_EACH_PAGE_MOVE_KERNEL(MI355_PAGE_MOVE_ROW)};
+typedef void (*page_finish_kernel_t)(PageFinishArgs);
+struct PageFinishVariant { unsigned nt_load, store; page_finish_kernel_t fn; };
+#define MI355_PAGE_FINISH_ROW(L, S) {L, S, mi355_pages_reserve_finish_l##L##_s##S},
+const PageFinishVariant kPageFinishVariants[] = {MI355_FOR_EACH_PAGE_FINISH_KERNEL(MI355_PAGE_FINISH_ROW)};
+
+PageMoveArgs page_move_args(const mi355_blit_pages& to, const mi355_blit_pages& from, const PageMovePlan& p,
+                            const int32_t* dst, const int32_t* src, const int32_t* valid, const PageMoveCount* count,
+                            uint64_t n) {
+  return {to.planes_dev[p.table], from.planes_dev[p.table], dst, src, valid, count,
+          magic_divisor(static_cast<uint32_t>(n)), static_cast<uint32_t>(n), to.pieces[p.table],
+          to.num_pages, from.num_pages, to.rows, p.grid * kMoveWaves};
+}
 
 // n moves, or the first *count of a list with room for n.
 int launch_page_moves(const mi355_blit_pages& to, const mi355_blit_pages& from, const int32_t* dst, const int32_t* src,
                       const int32_t* valid, const PageMoveCount* count, uint64_t n, uint32_t route, hipStream_t s) {
-  const PageMovePlan p = plan_page_moves(n, count != nullptr, valid != nullptr, to.pieces, to.page_bytes, to.h->num_cus,
-                                         route, kHostLinkMaxGrid);
+  const PageMovePlan p = plan_page_moves(n, count ? kMostListed : 0, valid != nullptr, to.pieces, to.page_bytes,
+                                         to.h->num_cus, route, kHostLinkMaxGrid);
   page_move_kernel_t k = nullptr;
   for (const PageMoveVariant& v : kPageMoveVariants)
     if (v.unroll == kPieceUnrolls[p.table] && v.nt_load == p.nt_load && v.store == p.store_policy) k = v.fn;
   if (!k) return MI355_BLIT_ERROR;
-  const PageMoveArgs a{to.planes_dev[p.table], from.planes_dev[p.table], dst, src, valid, count,
-                       magic_divisor(static_cast<uint32_t>(n)), static_cast<uint32_t>(n), to.pieces[p.table],
-                       to.num_pages, from.num_pages, to.rows, p.grid * kMoveWaves};
-  hipLaunchKernelGGL(k, dim3(p.grid), dim3(kMoveWaves * kWave), 0, s, a);
+  hipLaunchKernelGGL(k, dim3(p.grid), dim3(kMoveWaves * kWave), 0, s,
+                     page_move_args(to, from, p, dst, src, valid, count, n));
   BLIT_HIP(hipGetLastError());
   return MI355_BLIT_SUCCESS;
 }
@@ -946,13 +957,11 @@ int mi355_blit_pages_create(mi355_blit_t* h, const mi355_blit_pages_desc_t* desc
     p->has_book = true;
     p->book_words = at.words;
     p->book = pages_book_ptrs(desc->book, at, desc->num_pages, desc->max_seqs, desc->max_pages_per_seq, desc->rows);
-    // lists of moves: an entry of a reservation, or a pair of a compaction
-    const uint64_t room = desc->num_pages > 2 * kMaxList ? desc->num_pages / 2 : kMaxList;
-    const uint64_t words = 64 + 3 * room + desc->num_pages;
-    if (rc == MI355_BLIT_SUCCESS) e = hipMalloc(&p->work_dev, words * sizeof(int32_t));
+    const PageWorkLayout w = pages_work_layout(desc->num_pages);
+    if (rc == MI355_BLIT_SUCCESS) e = hipMalloc(&p->work_dev, w.words * sizeof(uint32_t));
     if (rc == MI355_BLIT_SUCCESS && e == hipSuccess) {
-      int32_t* w = static_cast<int32_t*>(p->work_dev);
-      p->moves = {w + 64, w + 64 + room, w + 64 + 2 * room, w + 64 + 3 * room, reinterpret_cast<PageMoveCount*>(w)};
+      p->moves = pages_move_list(static_cast<uint32_t*>(p->work_dev), w);
+      p->reserve = pages_reserve_work(static_cast<uint32_t*>(p->work_dev), w);
     }
   }
   std::free(table);
@@ -1022,11 +1031,24 @@ int mi355_blit_pages_reserve(mi355_blit_pages_t* p, const int32_t* seqs, const i
   DeviceScope scope(p->h->device);
   if (scope.err != hipSuccess) return status_of(scope.err);
   hipStream_t s = stream ? static_cast<hipStream_t>(stream) : p->h->stream;
-  const PageReserveArgs a{p->book, p->moves, seqs, more, granted, static_cast<uint32_t>(n), 0};
+  // at most a copy for each entry, and no more than there are pages
+  const uint64_t copies = n < p->num_pages ? n : p->num_pages;
+  const PageMovePlan m = plan_page_moves(copies, kMostReserved, true, p->pieces, p->page_bytes, p->h->num_cus,
+                                         MI355_BLIT_ROUTE_DEVICE, kHostLinkMaxGrid);
+  page_finish_kernel_t k = nullptr;
+  for (const PageFinishVariant& v : kPageFinishVariants)
+    if (v.nt_load == m.nt_load && v.store == m.store_policy) k = v.fn;
+  if (!k) return MI355_BLIT_ERROR;
+  const PageReserveArgs a{p->book, p->moves, p->reserve, seqs, more, granted, static_cast<uint32_t>(n),
+                          reserve_lane_vecs(p->num_pages)};
+  const uint32_t n_pairs = (p->num_pages + 63) / 64;
+  const uint32_t want = (n_pairs + kMoveWaves - 1) / kMoveWaves;
+  const PageFinishArgs f{page_move_args(*p, *p, m, p->moves.dst, p->moves.src, p->moves.valid, p->moves.count, copies),
+                         p->book, p->reserve, static_cast<uint32_t>(n), n_pairs, want < kMostAssign ? want : kMostAssign, 0};
   hipLaunchKernelGGL(mi355_pages_reserve, dim3(1), dim3(1024), 0, s, a);
+  hipLaunchKernelGGL(k, dim3(f.assign_wgs + m.grid), dim3(kMoveWaves * kWave), 0, s, f);
   BLIT_HIP(hipGetLastError());
-  return launch_page_moves(*p, *p, p->moves.dst, p->moves.src, p->moves.valid, p->moves.count,
-                           n < p->num_pages ? n : p->num_pages, MI355_BLIT_ROUTE_DEVICE, s);
+  return MI355_BLIT_SUCCESS;
 }
 
 int mi355_blit_pages_fork(mi355_blit_pages_t* p, const int32_t* parents, const int32_t* children, size_t n,

@@ -261,6 +261,9 @@ MI355_DEVICE uint32_t lane_read_up(uint32_t v, unsigned delta) { return __shfl_u
 // The value of the wave's first lane, as a wave-uniform (scalar) value.
 MI355_DEVICE uint32_t wave_uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 
+// The lanes (bit i: lane i) that passed true.
+MI355_DEVICE uint64_t wave_ballot(bool v) { return __ballot(v); }
+
 // Bytes r..r+3 of the little-endian pair {hi:lo}, r in 0..3.
 MI355_DEVICE unsigned shift_bytes(unsigned hi, unsigned lo, unsigned r) {
   return __builtin_amdgcn_alignbyte(hi, lo, r);

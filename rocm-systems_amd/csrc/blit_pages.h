@@ -90,13 +90,36 @@ struct PageMoveList {
   PageMoveCount* count;
 };
 
+// What the first launch of a reservation leaves for the second: for each entry
+// how many pages the entries before it get, the sequence (and whether its first
+// page takes the place of a shared one) and the first table slot, and for each
+// two words of the free bits how many free pages are in front of them.
+struct PageReserveWork {
+  uint32_t* start;
+  uint32_t* who;  // sequence, top bit: copies
+  uint32_t* slot;
+  uint32_t* pairs;
+  uint32_t* wanted;  // pages that the second launch hands out
+};
+
 struct PageReserveArgs {
   BookPtrs book;
   PageMoveList moves;
+  PageReserveWork work;
   const int32_t* seqs;
   const int32_t* add;
   int32_t* granted;  // may be null
   uint32_t n;
+  uint32_t lane_vecs;  // 16-byte vectors of free bits for each of 1024 lanes: a power of two
+};
+
+struct PageFinishArgs {
+  PageMoveArgs moves;
+  BookPtrs book;
+  PageReserveWork work;
+  uint32_t n;
+  uint32_t n_pairs;
+  uint32_t assign_wgs;  // workgroups that hand out pages; those behind them move
   uint32_t pad;
 };
 
@@ -130,6 +153,14 @@ struct PageResetArgs {
   uint64_t words;  // of the whole buffer
 };
 
+// The free bits as the first launch of a reservation takes them: one stretch
+// of 16-byte vectors for each of 1024 lanes.
+inline uint32_t reserve_lane_vecs(uint32_t num_pages) {
+  uint32_t v = 1;
+  while (static_cast<uint64_t>(v) * 1024 * 128 < num_pages) v *= 2;
+  return v;
+}
+
 // Sequences that one call can name, sequences and pages that a book can have.
 constexpr uint32_t kMaxList = MI355_BLIT_PAGES_MAX_LIST;
 constexpr uint32_t kMaxSeqs = MI355_BLIT_PAGES_MAX_SEQS;
@@ -156,6 +187,37 @@ inline BookPtrs pages_book_ptrs(int32_t* book, const mi355_blit_book_t& at, uint
                                 uint32_t width, uint32_t rows) {
   return {book, book + at.lengths, book + at.ref_counts, reinterpret_cast<uint32_t*>(book + at.free_bits),
           book + at.tables, num_pages, max_seqs, width, rows, magic_divisor(rows)};
+}
+
+// The work memory of a book's calls, in words.  Every word that a launch reads
+// was written by one before it in the same call.
+struct PageWorkLayout {
+  uint64_t move_src, move_dst, move_valid, remap, start, who, slot, pairs, words;
+};
+
+inline PageWorkLayout pages_work_layout(uint32_t num_pages) {
+  // a move for each entry of a reservation, or for each two pages of a compaction
+  const uint64_t moves = book_up(num_pages > 2 * kMaxList ? num_pages / 2 : kMaxList);
+  PageWorkLayout w;
+  w.move_src = kBookAlign;  // the count of moves and that of pages to hand out are in front
+  w.move_dst = w.move_src + moves;
+  w.move_valid = w.move_dst + moves;
+  w.remap = w.move_valid + kMaxList;
+  w.start = w.remap + book_up(num_pages);
+  w.who = w.start + kMaxList;
+  w.slot = w.who + kMaxList;
+  w.pairs = w.slot + kMaxList;
+  w.words = w.pairs + book_up((num_pages + 127ull) / 128 * 2);
+  return w;
+}
+
+inline PageMoveList pages_move_list(uint32_t* work, const PageWorkLayout& w) {
+  int32_t* p = reinterpret_cast<int32_t*>(work);
+  return {p + w.move_src, p + w.move_dst, p + w.move_valid, p + w.remap, reinterpret_cast<PageMoveCount*>(work)};
+}
+
+inline PageReserveWork pages_reserve_work(uint32_t* work, const PageWorkLayout& w) {
+  return {work + w.start, work + w.who, work + w.slot, work + w.pairs, work + 16};
 }
 
 inline uint64_t plane_page_bytes(const mi355_blit_plane_t& p, uint32_t rows) {
@@ -219,8 +281,8 @@ struct PageMovePlan {
   uint32_t nt_load, store_policy, grid;
 };
 
-// How n moves are launched; `listed`: n is what the list has room for, the
-// device knows how many there are.  pieces: of a page, for each size of piece.
+// How n moves are launched; most_per_cu not 0: n is what a list has room for,
+// the device knows how many there are, and this many workgroups for each CU are the most.  pieces: of a page, for each size of piece.
 //
 // Cache policy, by the bytes that are likely moved (half of the pages where only
 // their first rows are).  Measured, pages of 32 planes of 32 KiB, loads and stores cached /
@@ -236,11 +298,16 @@ struct PageMovePlan {
 // at most), and strides beyond (800 MiB 292 us; with 128 for each CU 325).
 // Over the host link at most link_grid workgroups, as for the linear copy; what
 // goes to the host is written through at once.
+// A reservation's list is as long as the call's and mostly empty: kMostReserved
+// for each CU (256 copies of 16 KiB in 32 planes 27.5 us, 25.5 with a wave for each piece,
+// which costs 6 us where nothing is copied).
 constexpr uint32_t kMoveWaves = 4;
-constexpr uint32_t kMostListed = 512;
+constexpr uint32_t kMostListed = 512, kMostReserved = 16;
+// Workgroups that hand out pages, 256 pages each at a time.
+constexpr uint32_t kMostAssign = 1024;
 constexpr uint64_t kMoveStreams = 128ull << 20, kMoveNtStores = 320ull << 20;
 
-inline PageMovePlan plan_page_moves(uint64_t n, bool listed, bool cut, const uint32_t (&pieces)[2], uint64_t page_bytes,
+inline PageMovePlan plan_page_moves(uint64_t n, uint32_t most_per_cu, bool cut, const uint32_t (&pieces)[2], uint64_t page_bytes,
                                     uint32_t num_cus, uint32_t route, uint32_t link_grid) {
   PageMovePlan p;
   p.table = cut ? 1 : 0;
@@ -251,7 +318,7 @@ inline PageMovePlan plan_page_moves(uint64_t n, bool listed, bool cut, const uin
                    : bytes >= kMoveStreams ? MI355_BLIT_STORE_AGENT_WT : MI355_BLIT_STORE_CACHED;
   const uint64_t want = (n * pieces[p.table] + kMoveWaves - 1) / kMoveWaves;
   const uint64_t most = route != MI355_BLIT_ROUTE_DEVICE ? link_grid
-                        : listed ? static_cast<uint64_t>(num_cus) * kMostListed : kMaxGridWorkItems / (kMoveWaves * kWave);
+                        : most_per_cu ? static_cast<uint64_t>(num_cus) * most_per_cu : kMaxGridWorkItems / (kMoveWaves * kWave);
   p.grid = static_cast<uint32_t>(want < most ? want : most);
   return p;
 }

@@ -67,7 +67,7 @@ MI355_DEVICE void move_piece(uint8_t* d, const uint8_t* s, const PagePlane& g, u
 }
 
 template <int U, bool NTL, int ST>
-MI355_DEVICE void page_move_body(const PageMoveArgs& a) {
+MI355_DEVICE void page_move_body(const PageMoveArgs& a, uint64_t first_wave) {
   const unsigned lane = thread_in_workgroup() & (kWave - 1);
   uint32_t n = a.n;
   uint64_t magic_n = a.magic_n;
@@ -77,7 +77,7 @@ MI355_DEVICE void page_move_body(const PageMoveArgs& a) {
   }
   // fits in 32 bits (checked on the host); the sum with n_waves may not
   const uint64_t total = static_cast<uint64_t>(n) * a.pieces;
-  for (uint64_t w = global_wave(kMoveWaves); w < total; w += a.n_waves) {
+  for (uint64_t w = first_wave; w < total; w += a.n_waves) {
     const uint32_t item = static_cast<uint32_t>(w);
     const uint32_t some_piece = div_magic(item, magic_n);
     const PagePlane d = ld_uniform_plane(a.dst_planes + some_piece);
@@ -152,52 +152,122 @@ MI355_DEVICE uint32_t hash_slot(uint32_t* keys, uint32_t key) {
   }
 }
 
-// Room for new tokens.  One workgroup of 1024 lanes takes the entries 1024 at
-// a time: which of them name a sequence first (a table in LDS, and a bit for each sequence
-// that an earlier round named), which of them have to copy a last page that
-// others hold as well, how many pages each needs, and from the free bits
-// which pages those are: the k-th lowest free page goes to the entry whose
-// share of the running sum of needs k falls into, so that the result is that of
-// taking the entries one by one.
+// A word of the free bits without the pages that do not exist.
+MI355_DEVICE uint32_t existing_bits(const BookPtrs& b, uint32_t word, uint32_t index) {
+  const uint32_t first = 32 * index;
+  if (first >= b.num_pages) return 0;
+  return b.num_pages - first >= 32 ? word : word & ((1u << (b.num_pages - first)) - 1);
+}
+
+// Vector v of the free bits, which may lie behind them.
+MI355_DEVICE BitTile load_bits_vec(const BookPtrs& b, uint32_t v) {
+  BitTile t{};
+  if (128 * v < b.num_pages) {
+    const v4u x = ld_v4<false>(reinterpret_cast<const v4u_a4*>(b.bits + 4 * v));
+    t.word[0] = existing_bits(b, x.x, 4 * v);
+    t.word[1] = existing_bits(b, x.y, 4 * v + 1);
+    t.word[2] = existing_bits(b, x.z, 4 * v + 2);
+    t.word[3] = existing_bits(b, x.w, 4 * v + 3);
+  }
+  return t;
+}
+
+// Place of the bit of `word` that has `r` set bits below it.
+MI355_DEVICE uint32_t nth_bit(uint32_t word, uint32_t r) {
+  uint32_t at = 0;
+#pragma unroll
+  for (uint32_t half = 16; half >= 1; half >>= 1) {
+    const uint32_t below = popcount32(word >> at & ((1u << half) - 1));
+    if (r >= below) r -= below, at += half;
+  }
+  return at;
+}
+
+// The free page with `rank` free pages below it; groups[g] is the number of
+// free pages in front of lane g's stretch.
+MI355_DEVICE uint32_t select_page(const BookPtrs& b, const uint32_t* groups, uint32_t lane_vecs, uint32_t rank) {
+  uint32_t g = 0;  // the last stretch that starts at or in front of it
+#pragma unroll
+  for (uint32_t step = 512; step >= 1; step >>= 1)
+    if (groups[g + step] <= rank) g += step;
+  uint32_t r = rank - groups[g];
+  for (uint32_t v = g * lane_vecs; v < (g + 1) * lane_vecs; ++v) {
+    const BitTile bits = load_bits_vec(b, v);
+#pragma unroll
+    for (unsigned k = 0; k < 4; ++k) {
+      const uint32_t here = popcount32(bits.word[k]);
+      if (r < here) return 32 * (4 * v + k) + nth_bit(bits.word[k], r);
+      r -= here;
+    }
+  }
+  return 0;  // not reached: the rank is below the number of free pages
+}
+
+// The page with rank nth goes to the entry whose share of the running sum of
+// needs nth falls into.
+MI355_DEVICE void hand_out(const BookPtrs& b, uint32_t page, uint32_t nth, uint32_t start, uint32_t who, uint32_t slot) {
+  const uint64_t row = static_cast<uint64_t>(who & 0x7fffffffu) * b.width;
+  st_obj(b.tables + row + slot + (nth - start), static_cast<int32_t>(page));
+  st_obj(b.refs + page, 1);
+}
+
+// Room for new tokens, in two launches, so that the result is that of taking
+// the entries one by one.
+//
+// The first, one workgroup of 1024 lanes, takes the entries 1024 at a time:
+// which of them name a sequence first (a table in LDS, and a bit for each
+// sequence that an earlier round named), which of them have to copy a last page
+// that others hold as well, how many pages each needs and how many the entries
+// before it get, out of how many free ones.  The k-th lowest free page goes to the
+// entry whose share of the running sum k falls into.  Where the pages are no
+// more than the lanes (a decode step), it hands them out itself, a lane for each page; otherwise
+// the second launch does, over the whole device, next to the copies.
 //
 // Bound by latency: a chain of dependent loads (entry, length, last page,
 // its count, free bits) and a dozen barriers.
 MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
-  constexpr uint32_t kIds = 2048;
   MI355_LDS uint32_t scan_a[16], scan_b[16];
   MI355_LDS uint32_t keys[kSlots], first[kSlots], asked[kSlots];
   MI355_LDS uint32_t seen[kMaxSeqs / 32];
-  MI355_LDS uint32_t start[1024], who[1024], slot_of[1024], tail_of[1024], fill_of[1024];
-  MI355_LDS uint32_t ids[kIds];
-  MI355_LDS uint32_t any_shared, any_refused, granted_pages, n_moves;
+  MI355_LDS uint32_t start[1024], who[1024], slot_of[1024], groups[1024];
+  MI355_LDS uint32_t any_shared, any_refused, handed, n_moves;
   const BookPtrs& b = a.book;
   const uint32_t t = thread_in_workgroup();
-  const uint32_t n_tiles = (b.num_pages + kTilePages - 1) / kTilePages;
 
+  // the free bits, a stretch for each lane
+  uint32_t mine = 0;
+  for (uint32_t k = 0; k < a.lane_vecs; ++k) mine += count_bits(load_bits_vec(b, t * a.lane_vecs + k));
   for (uint32_t k = t; k < kMaxSeqs / 32; k += 1024) seen[k] = 0;
-  if (t == 0) n_moves = 0;
-  uint32_t tile = 0;     // no free page in front of this tile
+  if (t == 0) n_moves = 0, handed = 0;
+  uint32_t free_pages;
+  const uint32_t in_front = block_scan_1024(mine, scan_b, &free_pages);
+  groups[t] = in_front;
+
   bool stopped = false;  // the same in all lanes
+  uint32_t carry = 0;    // pages that earlier rounds get
   for (uint32_t base = 0; base < a.n; base += 1024) {
     const uint32_t i = base + t;
     if (stopped) {
-      if (i < a.n && a.granted) st_obj(a.granted + i, 0);
+      if (i < a.n) {
+        if (a.granted) st_obj(a.granted + i, 0);
+        st_u32(a.work.start + i, ~0u);
+      }
       continue;
     }
-    for (uint32_t k = t; k < kSlots; k += 1024) keys[k] = kNoKey, first[k] = ~0u;
-    if (t == 0) any_shared = 0, any_refused = 0, granted_pages = 0;
-    workgroup_barrier();
-
     const uint32_t s = i < a.n ? static_cast<uint32_t>(ld_obj(a.seqs + i)) : ~0u;
     const int32_t more = i < a.n ? ld_obj(a.add + i) : 0;
+    for (uint32_t k = t; k < kSlots; k += 1024) keys[k] = kNoKey, first[k] = ~0u;
+    if (t == 0) any_shared = 0, any_refused = 0;
+    workgroup_barrier();
+
     const bool named = s < b.max_seqs;
     uint32_t slot = 0, tokens = 0;
     bool again = false;
     if (named) {
+      tokens = ld_obj(b.lengths + s);
       again = seen[s / 32] >> (s % 32) & 1;
       slot = hash_slot(keys, s);
       lds_min(first + slot, t);
-      tokens = ld_obj(b.lengths + s);
     }
     workgroup_barrier();
     if (named) {
@@ -214,6 +284,7 @@ MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
     if (ok && more > 0 && fill != 0) {
       tail = ld_obj(b.tables + static_cast<uint64_t>(s) * b.width + old_pages - 1);
       if (tail < b.num_pages) {
+        // an earlier round may have changed it
         holders = ld_agent_u32(reinterpret_cast<const uint32_t*>(b.refs + tail));
         shared = static_cast<int32_t>(holders) > 1;
       } else {
@@ -241,88 +312,105 @@ MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
     if (need > b.num_pages) need = b.num_pages + 1;
     uint32_t total;
     const uint32_t before = block_scan_1024(need, scan_a, &total);
-
-    // how many of them there are
-    uint32_t found = 0;
-    for (uint32_t k = tile; k < n_tiles && found < total; ++k) {
-      uint32_t here;
-      block_scan_1024(count_bits(load_bits(b, k)), scan_b, &here);
-      found += here;
-      workgroup_barrier();
-    }
-    const bool granted = ok && before + need <= found;
+    const bool granted = ok && before + need <= free_pages - carry;
     if (ok && !granted) any_refused = 1;
-    if (granted) lds_max(&granted_pages, before + need);
-    start[t] = before;
+    if (granted && need) lds_max(&handed, carry + before + need);
+    start[t] = carry + before;
     who[t] = s | (copies ? 1u << 31 : 0);
     slot_of[t] = old_pages - (copies ? 1 : 0);
-    tail_of[t] = tail;
-    fill_of[t] = fill;
     workgroup_barrier();
     stopped = any_refused != 0;
-    const uint32_t wanted = granted_pages;
-
-    // the pages, lowest first
-    uint32_t done = 0;
-    while (done < wanted) {
-      BitTile bits = load_bits(b, tile);
-      uint32_t here;
-      uint32_t rank = block_scan_1024(count_bits(bits), scan_b, &here);
-      workgroup_barrier();
-      const uint32_t take = here < wanted - done ? here : wanted - done;
-      const uint32_t w = tile * kTileWords + 4 * t;
-      unsigned k = 0;
-      bool changed = false;
-      for (uint32_t round = 0; round < take; round += kIds) {
-        const uint32_t end = take - round < kIds ? take : round + kIds;
-        while (k < 4 && rank < end) {
-          if (bits.word[k] == 0) {
-            ++k;
-            continue;
-          }
-          ids[rank - round] = 32 * (w + k) + lowest_bit(bits.word[k]);
-          bits.word[k] &= bits.word[k] - 1;
-          changed = true;
-          ++rank;
-        }
-        workgroup_barrier();
-        for (uint32_t q = round + t; q < end; q += 1024) {
-          const uint32_t page = ids[q - round];
-          const uint32_t nth = done + q;
-          uint32_t e = 0;  // the last entry that starts at or in front of nth
-#pragma unroll
-          for (uint32_t step = 512; step >= 1; step >>= 1)
-            if (start[e + step] <= nth) e += step;
-          const uint32_t seq = who[e] & 0x7fffffffu;
-          const uint32_t j = nth - start[e];
-          st_obj(b.tables + static_cast<uint64_t>(seq) * b.width + slot_of[e] + j, static_cast<int32_t>(page));
-          st_obj(b.refs + page, 1);
-          if (j == 0 && who[e] >> 31) {
-            const uint32_t m = lds_add(&n_moves, 1);
-            st_obj(a.moves.src + m, static_cast<int32_t>(tail_of[e]));
-            st_obj(a.moves.dst + m, static_cast<int32_t>(page));
-            st_obj(a.moves.valid + m, static_cast<int32_t>(fill_of[e]));
-            add_agent_i32(b.refs + tail_of[e], -1);
-          }
-        }
-        workgroup_barrier();
-      }
-      if (changed) {
-        // words behind the last page are not written
-#pragma unroll
-        for (unsigned c = 0; c < 4; ++c)
-          if (32 * (w + c) < b.num_pages) st_u32(b.bits + w + c, bits.word[c]);
-      }
-      done += take;
-      if (done < wanted) ++tile;
+    const uint32_t wanted = handed;  // up to here
+    if (granted && copies) {
+      const uint32_t m = lds_add(&n_moves, 1);
+      st_obj(a.moves.src + m, static_cast<int32_t>(tail));
+      st_obj(a.moves.dst + m, static_cast<int32_t>(select_page(b, groups, a.lane_vecs, carry + before)));
+      st_obj(a.moves.valid + m, static_cast<int32_t>(fill));
+      add_agent_i32(b.refs + tail, -1);
     }
     if (granted && more > 0) st_obj(b.lengths + s, static_cast<int32_t>(tokens + more));
     if (i < a.n && a.granted) st_obj(a.granted + i, granted ? 1 : 0);
-    // the next round reads counts and bits that this one wrote
-    wait_for_memory();
+    if (a.n <= 1024 && wanted <= 1024) {
+      if (t < wanted) {
+        uint32_t e = 0;  // the last entry that starts at or in front of the lane's page
+#pragma unroll
+        for (uint32_t step = 512; step >= 1; step >>= 1)
+          if (start[e + step] <= t) e += step;
+        const uint32_t page = select_page(b, groups, a.lane_vecs, t);
+        hand_out(b, page, t, start[e], who[e], slot_of[e]);
+        tail = page;  // kept for below
+      }
+      // every lane has read the bits it needs
+      workgroup_barrier();
+      if (t < wanted) and_agent_u32(b.bits + tail / 32, ~(1u << (tail % 32)));
+      if (t == 0) handed = 0;
+    } else {
+      if (i < a.n) {
+        st_u32(a.work.start + i, start[t]);
+        st_u32(a.work.who + i, who[t]);
+        st_u32(a.work.slot + i, slot_of[t]);
+      }
+      carry = wanted;
+      // the next round reads counts that this one wrote
+      wait_for_memory();
+    }
     workgroup_barrier();
   }
-  if (t == 0) st_obj(a.moves.count, PageMoveCount{n_moves, 0, magic_divisor(n_moves)});
+  if (handed) {
+    uint32_t front = in_front;
+    for (uint32_t k = 0; k < a.lane_vecs; ++k) {
+      const uint32_t v = t * a.lane_vecs + k;
+      if (128 * v >= b.num_pages) break;
+      const BitTile bits = load_bits_vec(b, v);
+      st_u32(a.work.pairs + 2 * v, front);
+      front += popcount32(bits.word[0]) + popcount32(bits.word[1]);
+      st_u32(a.work.pairs + 2 * v + 1, front);
+      front += popcount32(bits.word[2]) + popcount32(bits.word[3]);
+    }
+  }
+  if (t == 0) {
+    st_obj(a.moves.count, PageMoveCount{n_moves, 0, magic_divisor(n_moves)});
+    st_u32(a.work.wanted, handed);
+  }
+}
+
+// The second launch hands out what the first has left, a wave for 64 pages at
+// a time, a lane for each; the entry that a page goes to is found by bisection
+// of the running sum.
+MI355_DEVICE void page_assign_body(const PageFinishArgs& a) {
+  const BookPtrs& b = a.book;
+  const unsigned lane = thread_in_workgroup() & (kWave - 1);
+  const uint32_t wanted = ld_uniform_u32(a.work.wanted);
+  for (uint32_t pair = static_cast<uint32_t>(global_wave(kMoveWaves)); pair < a.n_pairs; pair += a.assign_wgs * kMoveWaves) {
+    if (wanted == 0) return;
+    const uint32_t front = ld_uniform_u32(a.work.pairs + pair);
+    if (front >= wanted) return;  // and so it is for every later pair
+    const uint32_t index = 2 * pair + lane / 32;
+    uint32_t word = 0;
+    if (32 * index < b.num_pages) word = existing_bits(b, ld_u32<false>(b.bits + index), index);
+    const uint32_t low = lane_read(word, 0);
+    const uint32_t nth = front + (lane < 32 ? 0 : popcount32(low)) + popcount32(word & ((1u << (lane % 32)) - 1));
+    const bool taken = (word >> (lane % 32) & 1) && nth < wanted;
+    if (taken) {
+      uint32_t e = 0;
+#pragma unroll
+      for (uint32_t step = kMaxList / 2; step >= 1; step >>= 1)
+        if (e + step < a.n && ld_u32<false>(a.work.start + e + step) <= nth) e += step;
+      hand_out(b, 32 * index + lane % 32, nth, ld_u32<false>(a.work.start + e), ld_u32<false>(a.work.who + e),
+               ld_u32<false>(a.work.slot + e));
+    }
+    const uint64_t gone = wave_ballot(taken);
+    const uint32_t mine = lane < 32 ? static_cast<uint32_t>(gone) : static_cast<uint32_t>(gone >> 32);
+    if (lane % 32 == 0 && mine) st_u32(b.bits + index, word & ~mine);
+  }
+}
+
+template <bool NTL, int ST>
+MI355_DEVICE void page_finish_body(const PageFinishArgs& a) {
+  if (workgroup_index() < a.assign_wgs)
+    page_assign_body(a);
+  else
+    page_move_body<4, NTL, ST>(a.moves, global_wave(kMoveWaves) - a.assign_wgs * kMoveWaves);
 }
 
 // A sequence that holds its parent's pages.  A workgroup of 256 lanes for each
@@ -510,9 +598,17 @@ MI355_DEVICE void page_reset_body(const PageResetArgs& a) {
 #define MI355_FOR_EACH_PAGE_MOVE_KERNEL(X) MI355_PAGE_MOVE_LS_(X, 1) MI355_PAGE_MOVE_LS_(X, 4)
 #define MI355_DEFINE_PAGE_MOVE(U, L, S)                                                       \
   MI355_KERNEL(256) void mi355_pages_move_u##U##_l##L##_s##S(mi355::PageMoveArgs a) {         \
-    mi355::page_move_body<U, L != 0, S>(a);                                                   \
+    mi355::page_move_body<U, L != 0, S>(a, mi355::global_wave(mi355::kMoveWaves));            \
   }
 MI355_FOR_EACH_PAGE_MOVE_KERNEL(MI355_DEFINE_PAGE_MOVE)
+
+//   mi355_pages_reserve_finish_l<nt loads>_s<store policy>
+#define MI355_FOR_EACH_PAGE_FINISH_KERNEL(X) X(0, 0) X(1, 1) X(1, 2)
+#define MI355_DEFINE_PAGE_FINISH(L, S)                                                        \
+  MI355_KERNEL(256) void mi355_pages_reserve_finish_l##L##_s##S(mi355::PageFinishArgs a) {    \
+    mi355::page_finish_body<L != 0, S>(a);                                                    \
+  }
+MI355_FOR_EACH_PAGE_FINISH_KERNEL(MI355_DEFINE_PAGE_FINISH)
 
 MI355_KERNEL(1024) void mi355_pages_reserve(mi355::PageReserveArgs a) { mi355::page_reserve_body(a); }
 MI355_KERNEL(256) void mi355_pages_fork(mi355::PageForkArgs a) { mi355::page_fork_body(a); }

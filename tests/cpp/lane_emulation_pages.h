@@ -53,6 +53,15 @@ MI355_DEVICE uint32_t lds_min(uint32_t* p, uint32_t v) { const uint32_t was = *p
 MI355_DEVICE uint32_t lds_max(uint32_t* p, uint32_t v) { const uint32_t was = *p; if (v > was) *p = v; return was; }
 MI355_DEVICE uint32_t lds_or(uint32_t* p, uint32_t v) { const uint32_t was = *p; *p |= v; return was; }
 
+MI355_DEVICE uint64_t wave_ballot(bool v) {
+  const unsigned parity = lane_emu::lane_move_arrive(v);
+  const lane_emu::Wave& w = lane_emu::g_m.waves[lane_emu::g_m.cur / kWave];
+  uint64_t all = 0;
+  for (unsigned i = 0; i < kWave; ++i)
+    if (w.deposited[parity] >> i & 1 && w.operand[parity][i]) all |= 1ull << i;
+  return all;
+}
+
 MI355_DEVICE unsigned popcount32(uint32_t v) { return static_cast<unsigned>(__builtin_popcount(v)); }
 MI355_DEVICE unsigned lowest_bit(uint32_t v) { return static_cast<unsigned>(__builtin_ctz(v)); }
 

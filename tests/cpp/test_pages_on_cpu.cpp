@@ -140,13 +140,14 @@ struct Cache {
   int32_t* book = nullptr;
   BookPtrs ptrs;
   PageMoveList moves;
-  std::vector<int32_t> work;
-  uint64_t room;
+  PageReserveWork reserving;
+  uint32_t* work = nullptr;
+  uint64_t work_words = 0;
   // the book as it should be
   List lengths, refs, tables;
   int32_t head = 0;
 
-  ~Cache() { std::free(book); }
+  ~Cache() { std::free(book), std::free(work); }
 
   bool make(const Config& c) {
     if (!pool.make(c, true)) return false;
@@ -156,10 +157,13 @@ struct Cache {
     book = static_cast<int32_t*>(q);
     for (uint64_t i = 0; i < at.words; ++i) book[i] = static_cast<int32_t>(rnd());
     ptrs = pages_book_ptrs(book, at, c.pages, c.seqs, c.width, c.rows);
-    room = c.pages > 2 * kMaxList ? c.pages / 2 : kMaxList;
-    work.assign(64 + 3 * room + c.pages, 0x55555555);
-    int32_t* w = work.data();
-    moves = {w + 64, w + 64 + room, w + 64 + 2 * room, w + 64 + 3 * room, reinterpret_cast<PageMoveCount*>(w)};
+    const PageWorkLayout w = pages_work_layout(c.pages);
+    work_words = w.words;
+    if (posix_memalign(&q, 256, work_words * 4)) std::abort();
+    work = static_cast<uint32_t*>(q);
+    for (uint64_t i = 0; i < work_words; ++i) work[i] = static_cast<uint32_t>(rnd());
+    moves = pages_move_list(work, w);
+    reserving = pages_reserve_work(work, w);
     start();
     run(mi355_pages_reset, PageResetArgs{ptrs, at.words}, static_cast<uint32_t>((at.words + 255) / 256), 256);
     lengths.assign(c.seqs, 0);
@@ -176,8 +180,8 @@ struct Cache {
     g_check.clear();
     g_check.allow_read(book, at.words * 4);
     g_check.allow_write(book, at.words * 4);
-    g_check.allow_read(work.data(), work.size() * 4);
-    g_check.allow_write(work.data(), work.size() * 4);
+    g_check.allow_read(work, work_words * 4);
+    g_check.allow_write(work, work_words * 4);
     pool.allow(true);
   }
   void reads(const Words& w) { g_check.allow_read(w.p.get(), w.n * 4); }
@@ -195,7 +199,7 @@ struct Cache {
 
   static void run_moves(const Pool& to, const Pool& from, const int32_t* dst, const int32_t* src, const int32_t* valid,
                         const PageMoveCount* count, uint64_t n, uint32_t route, uint32_t cus) {
-    PageMovePlan p = plan_page_moves(n, count != nullptr, valid != nullptr, to.pieces, to.page_bytes, cus, route, 3);
+    PageMovePlan p = plan_page_moves(n, count ? 2 : 0, valid != nullptr, to.pieces, to.page_bytes, cus, route, 3);
     // the sizes here are small: the policies of large moves, and grids that stride
     if (p.store_policy == MI355_BLIT_STORE_CACHED && below(2)) p.nt_load = 1, p.store_policy = 1 + below(2);
     if (p.store_policy == MI355_BLIT_STORE_SYSTEM_WT) p.nt_load = below(2);
@@ -209,6 +213,24 @@ struct Cache {
     MI355_FOR_EACH_PAGE_MOVE_KERNEL(TRY)
 #undef TRY
     fail("no kernel for the plan");
+  }
+
+  void run_reserve(const Words& seqs, const Words& more, int32_t* granted, uint32_t n) {
+    if (!n) return;
+    run(mi355_pages_reserve, PageReserveArgs{ptrs, moves, reserving, seqs.p.get(), more.p.get(), granted, n,
+                                             reserve_lane_vecs(pool.c.pages)}, 1, 1024);
+    const uint64_t copies = n < pool.c.pages ? n : pool.c.pages;
+    const PageMovePlan p = plan_page_moves(copies, 2, true, pool.pieces, pool.page_bytes, 1 + below(3), 0, 3);
+    const uint32_t n_pairs = (pool.c.pages + 63) / 64;
+    const PageFinishArgs f{{pool.table[1], pool.table[1], moves.dst, moves.src, moves.valid, moves.count,
+                            magic_divisor(static_cast<uint32_t>(copies)), static_cast<uint32_t>(copies), pool.pieces[1],
+                            pool.c.pages, pool.c.pages, pool.c.rows, p.grid * kMoveWaves},
+                           ptrs, reserving, n, n_pairs, 1 + static_cast<uint32_t>(below((n_pairs + 3) / 4)), 0};
+    switch (below(3)) {
+      case 0: return run(mi355_pages_reserve_finish_l0_s0, f, f.assign_wgs + p.grid, 256);
+      case 1: return run(mi355_pages_reserve_finish_l1_s1, f, f.assign_wgs + p.grid, 256);
+      default: return run(mi355_pages_reserve_finish_l1_s2, f, f.assign_wgs + p.grid, 256);
+    }
   }
 
   void check(const char* what) {
@@ -229,8 +251,7 @@ struct Cache {
     Words s(seqs), m(more), granted(List(n, 77));
     start(), reads(s), reads(m), writes(granted);
     const bool tell = rnd() % 4 != 0;
-    run(mi355_pages_reserve, PageReserveArgs{ptrs, moves, s.p.get(), m.p.get(), tell ? granted.p.get() : nullptr, n, 0}, 1, 1024);
-    run_moves(pool, pool, moves.dst, moves.src, moves.valid, moves.count, n < pool.c.pages ? n : pool.c.pages, 0, 1 + below(3));
+    run_reserve(s, m, tell ? granted.p.get() : nullptr, n);
     // one entry after the other
     const auto before = pool.want;
     std::set<int32_t> named;
@@ -447,8 +468,7 @@ void random_words() {
       x.push_back(static_cast<int32_t>(below(4) ? below(c.seqs) : rnd())), y.push_back(static_cast<int32_t>(below(4) ? below(c.seqs) : rnd()));
     Words a(x), b(y), granted(List(n, 0)), out(List(c.pages + 2, 0));
     cache.start(), cache.reads(a), cache.reads(b), cache.writes(granted), cache.writes(out);
-    Cache::run(mi355_pages_reserve, PageReserveArgs{cache.ptrs, cache.moves, a.p.get(), b.p.get(), granted.p.get(), n, 0}, 1, 1024);
-    Cache::run_moves(cache.pool, cache.pool, cache.moves.dst, cache.moves.src, cache.moves.valid, cache.moves.count, n < c.pages ? n : c.pages, 0, 2);
+    cache.run_reserve(a, b, granted.p.get(), n);
     Cache::run(mi355_pages_fork, PageForkArgs{cache.ptrs, a.p.get(), b.p.get(), granted.p.get(), n, 0}, n, 256);
     Cache::run(mi355_pages_free, PageFreeArgs{cache.ptrs, a.p.get(), b.p.get(), n, 0}, n, 256);
     if (c.pages / 2) {
