@@ -375,7 +375,7 @@ int mi355_blit_plan_rect_route(const mi355_pitched_ptr_t* dst, const mi355_dim3_
  *
  * Everything a call reads or writes is in the GPU's memory (lists of sequences
  * and of pages, counts, what was granted), nothing is read back, and nothing is
- * allocated: a call is one to four kernel launches and may be recorded into a HIP graph.
+ * allocated: a call is one to three kernel launches and may be recorded into a HIP graph.
  * Lists are arrays of int32_t; a number that is out of range (-1, say) is an
  * entry to pass over.  They are read when the commands run and have to stay as
  * they are until then.  Calls on one pool use its book and its work memory: those that may overlap --

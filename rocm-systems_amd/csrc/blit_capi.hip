@@ -881,6 +881,11 @@ typedef void (*page_finish_kernel_t)(PageFinishArgs);
 struct PageFinishVariant { unsigned nt_load, store; page_finish_kernel_t fn; };
 #define MI355_PAGE_FINISH_ROW(L, S) {L, S, mi355_pages_reserve_finish_l##L##_s##S},
 const PageFinishVariant kPageFinishVariants[] = {MI355_FOR_EACH_PAGE_FINISH_KERNEL(MI355_PAGE_FINISH_ROW)};
+typedef void (*page_compact_finish_kernel_t)(PageCompactFinishArgs);
+struct PageCompactFinishVariant { unsigned nt_load, store; page_compact_finish_kernel_t fn; };
+#define MI355_PAGE_COMPACT_FINISH_ROW(L, S) {L, S, mi355_pages_compact_finish_l##L##_s##S},
+const PageCompactFinishVariant kPageCompactFinishVariants[] = {
+    MI355_FOR_EACH_PAGE_FINISH_KERNEL(MI355_PAGE_COMPACT_FINISH_ROW)};
 
 PageMoveArgs page_move_args(const mi355_blit_pages& to, const mi355_blit_pages& from, const PageMovePlan& p,
                             const int32_t* dst, const int32_t* src, const int32_t* valid, const PageMoveCount* count,
@@ -890,17 +895,16 @@ PageMoveArgs page_move_args(const mi355_blit_pages& to, const mi355_blit_pages& 
           to.num_pages, from.num_pages, to.rows, p.grid * kMoveWaves};
 }
 
-// n moves, or the first *count of a list with room for n.
 int launch_page_moves(const mi355_blit_pages& to, const mi355_blit_pages& from, const int32_t* dst, const int32_t* src,
-                      const int32_t* valid, const PageMoveCount* count, uint64_t n, uint32_t route, hipStream_t s) {
-  const PageMovePlan p = plan_page_moves(n, count ? kMostListed : 0, valid != nullptr, to.pieces, to.page_bytes,
-                                         to.h->num_cus, route, kHostLinkMaxGrid);
+                      const int32_t* valid, uint64_t n, uint32_t route, hipStream_t s) {
+  const PageMovePlan p = plan_page_moves(n, 0, valid != nullptr, to.pieces, to.page_bytes, to.h->num_cus, route,
+                                         kHostLinkMaxGrid);
   page_move_kernel_t k = nullptr;
   for (const PageMoveVariant& v : kPageMoveVariants)
     if (v.unroll == kPieceUnrolls[p.table] && v.nt_load == p.nt_load && v.store == p.store_policy) k = v.fn;
   if (!k) return MI355_BLIT_ERROR;
   hipLaunchKernelGGL(k, dim3(p.grid), dim3(kMoveWaves * kWave), 0, s,
-                     page_move_args(to, from, p, dst, src, valid, count, n));
+                     page_move_args(to, from, p, dst, src, valid, nullptr, n));
   BLIT_HIP(hipGetLastError());
   return MI355_BLIT_SUCCESS;
 }
@@ -1019,7 +1023,7 @@ int mi355_blit_pages_copy(mi355_blit_pages_t* dst, const int32_t* dst_pages, mi3
   std::lock_guard<std::mutex> g(dst->h->lock);
   DeviceScope scope(dst->h->device);
   if (scope.err != hipSuccess) return status_of(scope.err);
-  return launch_page_moves(*dst, *src, dst_pages, src_pages, valid_rows, nullptr, n, route,
+  return launch_page_moves(*dst, *src, dst_pages, src_pages, valid_rows, n, route,
                            stream ? static_cast<hipStream_t>(stream) : dst->h->stream);
 }
 
@@ -1041,10 +1045,9 @@ int mi355_blit_pages_reserve(mi355_blit_pages_t* p, const int32_t* seqs, const i
   if (!k) return MI355_BLIT_ERROR;
   const PageReserveArgs a{p->book, p->moves, p->reserve, seqs, more, granted, static_cast<uint32_t>(n),
                           reserve_lane_vecs(p->num_pages)};
-  const uint32_t n_pairs = (p->num_pages + 63) / 64;
-  const uint32_t want = (n_pairs + kMoveWaves - 1) / kMoveWaves;
   const PageFinishArgs f{page_move_args(*p, *p, m, p->moves.dst, p->moves.src, p->moves.valid, p->moves.count, copies),
-                         p->book, p->reserve, static_cast<uint32_t>(n), n_pairs, want < kMostAssign ? want : kMostAssign, 0};
+                         p->book, p->reserve, static_cast<uint32_t>(n), page_pairs(p->num_pages),
+                         page_pair_wgs(p->num_pages), 0};
   hipLaunchKernelGGL(mi355_pages_reserve, dim3(1), dim3(1024), 0, s, a);
   hipLaunchKernelGGL(k, dim3(f.assign_wgs + m.grid), dim3(kMoveWaves * kWave), 0, s, f);
   BLIT_HIP(hipGetLastError());
@@ -1058,9 +1061,13 @@ int mi355_blit_pages_fork(mi355_blit_pages_t* p, const int32_t* parents, const i
   std::lock_guard<std::mutex> g(p->h->lock);
   DeviceScope scope(p->h->device);
   if (scope.err != hipSuccess) return status_of(scope.err);
-  const PageForkArgs a{p->book, parents, children, granted, static_cast<uint32_t>(n), 0};
-  hipLaunchKernelGGL(mi355_pages_fork, dim3(static_cast<uint32_t>(n)), dim3(256), 0,
-                     stream ? static_cast<hipStream_t>(stream) : p->h->stream, a);
+  hipStream_t s = stream ? static_cast<hipStream_t>(stream) : p->h->stream;
+  const uint32_t wg = table_wg_size(p->book.width);
+  const bool split = p->book.width > kSplitWidth;
+  const uint32_t count = static_cast<uint32_t>(n);
+  const PageForkArgs a{p->book, parents, children, granted, split ? p->reserve.start : nullptr, count, wg};
+  hipLaunchKernelGGL(mi355_pages_fork, dim3(split ? count * table_chunks(p->book.width) : count), dim3(wg), 0, s, a);
+  if (split) hipLaunchKernelGGL(mi355_pages_fork_lengths, dim3((count + 255) / 256), dim3(256), 0, s, a);
   BLIT_HIP(hipGetLastError());
   return MI355_BLIT_SUCCESS;
 }
@@ -1071,9 +1078,17 @@ int mi355_blit_pages_free(mi355_blit_pages_t* p, const int32_t* seqs, const int3
   std::lock_guard<std::mutex> g(p->h->lock);
   DeviceScope scope(p->h->device);
   if (scope.err != hipSuccess) return status_of(scope.err);
-  const PageFreeArgs a{p->book, seqs, keep, static_cast<uint32_t>(n), 0};
-  hipLaunchKernelGGL(mi355_pages_free, dim3(static_cast<uint32_t>(n)), dim3(256), 0,
-                     stream ? static_cast<hipStream_t>(stream) : p->h->stream, a);
+  hipStream_t s = stream ? static_cast<hipStream_t>(stream) : p->h->stream;
+  const uint32_t wg = table_wg_size(p->book.width);
+  const uint32_t count = static_cast<uint32_t>(n);
+  const PageFreeArgs a{p->book, seqs, keep, count, wg};
+  if (n * p->book.width < kFreeByCounts && p->book.width <= kSplitWidth) {
+    hipLaunchKernelGGL(mi355_pages_free, dim3(count), dim3(wg), 0, s, a);
+  } else {
+    const uint32_t lanes = p->num_pages > count ? p->num_pages : count;
+    hipLaunchKernelGGL(mi355_pages_free_counts, dim3(count * table_chunks(p->book.width)), dim3(wg), 0, s, a);
+    hipLaunchKernelGGL(mi355_pages_free_finish, dim3((lanes + 255) / 256), dim3(256), 0, s, a);
+  }
   BLIT_HIP(hipGetLastError());
   return MI355_BLIT_SUCCESS;
 }
@@ -1087,12 +1102,21 @@ int mi355_blit_pages_compact(mi355_blit_pages_t* p, uint32_t max_moves, int32_t*
   DeviceScope scope(p->h->device);
   if (scope.err != hipSuccess) return status_of(scope.err);
   hipStream_t s = stream ? static_cast<hipStream_t>(stream) : p->h->stream;
-  const PageCompactArgs a{p->book, p->moves, moves, most, 0};
+  const PageMovePlan m = plan_page_moves(most, kMostListed, false, p->pieces, p->page_bytes, p->h->num_cus,
+                                         MI355_BLIT_ROUTE_DEVICE, kHostLinkMaxGrid);
+  page_compact_finish_kernel_t k = nullptr;
+  for (const PageCompactFinishVariant& v : kPageCompactFinishVariants)
+    if (v.nt_load == m.nt_load && v.store == m.store_policy) k = v.fn;
+  if (!k) return MI355_BLIT_ERROR;
+  const PageCompactArgs a{p->book, p->moves, p->reserve.pairs, p->reserve.wanted, moves, most,
+                          reserve_lane_vecs(p->num_pages), page_pairs(p->num_pages), page_pair_wgs(p->num_pages)};
+  const PageCompactFinishArgs f{
+      page_move_args(*p, *p, m, p->moves.dst, p->moves.src, nullptr, p->moves.count, most), a};
   hipLaunchKernelGGL(mi355_pages_compact_plan, dim3(1), dim3(1024), 0, s, a);
-  hipLaunchKernelGGL(mi355_pages_compact_apply, dim3((most + 255) / 256), dim3(256), 0, s, a);
-  hipLaunchKernelGGL(mi355_pages_compact_tables, dim3(p->book.max_seqs), dim3(256), 0, s, a);
+  if (most > kListedAtOnce) hipLaunchKernelGGL(mi355_pages_compact_list, dim3(a.pair_wgs), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(k, dim3(a.pair_wgs + p->book.max_seqs + m.grid), dim3(256), 0, s, f);
   BLIT_HIP(hipGetLastError());
-  return launch_page_moves(*p, *p, p->moves.dst, p->moves.src, nullptr, p->moves.count, most, MI355_BLIT_ROUTE_DEVICE, s);
+  return MI355_BLIT_SUCCESS;
 }
 
 namespace {

@@ -128,8 +128,9 @@ struct PageForkArgs {
   const int32_t* parents;
   const int32_t* children;
   int32_t* granted;  // may be null
+  uint32_t* made;    // not null: the children's lengths for the second launch
   uint32_t n;
-  uint32_t pad;
+  uint32_t wg_size;
 };
 
 struct PageFreeArgs {
@@ -137,15 +138,24 @@ struct PageFreeArgs {
   const int32_t* seqs;
   const int32_t* keep;  // null: 0
   uint32_t n;
-  uint32_t pad;
+  uint32_t wg_size;
 };
 
 struct PageCompactArgs {
   BookPtrs book;
   PageMoveList moves;
-  int32_t* out;  // [max_moves][2]: from, to; may be null
+  uint32_t* pairs;  // free pages in front of each two words of the free bits
+  uint32_t* live;   // pages in use
+  int32_t* out;     // [max_moves][2]: from, to; may be null
   uint32_t max_moves;
-  uint32_t pad;
+  uint32_t lane_vecs;  // as in PageReserveArgs
+  uint32_t n_pairs;
+  uint32_t pair_wgs;   // workgroups that go through the pairs
+};
+
+struct PageCompactFinishArgs {
+  PageMoveArgs moves;
+  PageCompactArgs compact;
 };
 
 struct PageResetArgs {
@@ -153,8 +163,8 @@ struct PageResetArgs {
   uint64_t words;  // of the whole buffer
 };
 
-// The free bits as the first launch of a reservation takes them: one stretch
-// of 16-byte vectors for each of 1024 lanes.
+// The free bits as the first launch of a reservation or a compaction takes
+// them: one stretch of 16-byte vectors for each of 1024 lanes.
 inline uint32_t reserve_lane_vecs(uint32_t num_pages) {
   uint32_t v = 1;
   while (static_cast<uint64_t>(v) * 1024 * 128 < num_pages) v *= 2;
@@ -276,6 +286,30 @@ inline uint32_t pages_planes(const mi355_blit_pages_desc_t& d, unsigned unroll, 
   return first;
 }
 
+// Lanes for each entry of a call that goes through tables of `width` pages, four
+// at a time.
+inline uint32_t table_wg_size(uint32_t width) { return width <= 1024 ? 256 : 1024; }
+// Pages of a table that one workgroup goes through where an entry has several,
+// and the width from which on it has.
+constexpr uint32_t kTableChunk = 4096;
+constexpr uint32_t kSplitWidth = 2 * kTableChunk;
+inline uint32_t table_chunks(uint32_t width) { return (width + kTableChunk - 1) / kTableChunk; }
+
+// From so many pages that a list can free on, the free bits are made from the
+// counts: 256 sequences of 375 pages (width 512) 14.4 us with an atomic for each
+// page's bit, 10.8 so; 128 sequences 12.3 and 11.1; 100 in tables of 700 8.5 and 11.5.
+constexpr uint64_t kFreeByCounts = 1u << 17;
+
+// Moves of a compaction that its first launch finds by itself.
+constexpr uint32_t kListedAtOnce = 1024;
+
+// Workgroups that go through all pages, 256 at a time.
+inline uint32_t page_pairs(uint32_t num_pages) { return (num_pages + 63) / 64; }
+inline uint32_t page_pair_wgs(uint32_t num_pages) {
+  const uint32_t want = (num_pages + 255) / 256;
+  return want < 1024 ? want : 1024;
+}
+
 struct PageMovePlan {
   uint32_t table;  // index into kPieceUnrolls
   uint32_t nt_load, store_policy, grid;
@@ -303,8 +337,6 @@ struct PageMovePlan {
 // which costs 6 us where nothing is copied).
 constexpr uint32_t kMoveWaves = 4;
 constexpr uint32_t kMostListed = 512, kMostReserved = 16;
-// Workgroups that hand out pages, 256 pages each at a time.
-constexpr uint32_t kMostAssign = 1024;
 constexpr uint64_t kMoveStreams = 128ull << 20, kMoveNtStores = 320ull << 20;
 
 inline PageMovePlan plan_page_moves(uint64_t n, uint32_t most_per_cu, bool cut, const uint32_t (&pieces)[2], uint64_t page_bytes,

@@ -107,32 +107,10 @@ MI355_DEVICE uint32_t pages_held(uint32_t tokens, const BookPtrs& b) {
   return div_magic(tokens, b.magic_rows) + (tokens - div_magic(tokens, b.magic_rows) * b.rows ? 1 : 0);
 }
 
-// A tile of the free bits: four words for each of the 1024 lanes.  Bits of
-// pages that do not exist are taken as 0 whatever the buffer holds.
-constexpr uint32_t kTileWords = 4 * 1024;
-constexpr uint32_t kTilePages = 32 * kTileWords;
-
+// Four words of the free bits.
 struct BitTile {
   uint32_t word[4];
 };
-
-MI355_DEVICE BitTile load_bits(const BookPtrs& b, uint32_t tile) {
-  BitTile t;
-  const uint32_t w = tile * kTileWords + 4 * thread_in_workgroup();
-#pragma unroll
-  for (unsigned k = 0; k < 4; ++k) t.word[k] = 0;
-  if (w * 32 < b.num_pages) {
-    const v4u v = ld_v4<false>(reinterpret_cast<const v4u_a4*>(b.bits + w));
-    t.word[0] = v.x, t.word[1] = v.y, t.word[2] = v.z, t.word[3] = v.w;
-#pragma unroll
-    for (unsigned k = 0; k < 4; ++k) {
-      const uint32_t first = 32 * (w + k);
-      if (first >= b.num_pages) t.word[k] = 0;
-      else if (b.num_pages - first < 32) t.word[k] &= (1u << (b.num_pages - first)) - 1;
-    }
-  }
-  return t;
-}
 
 MI355_DEVICE uint32_t count_bits(const BitTile& t) {
   return popcount32(t.word[0]) + popcount32(t.word[1]) + popcount32(t.word[2]) + popcount32(t.word[3]);
@@ -183,24 +161,29 @@ MI355_DEVICE uint32_t nth_bit(uint32_t word, uint32_t r) {
   return at;
 }
 
-// The free page with `rank` free pages below it; groups[g] is the number of
-// free pages in front of lane g's stretch.
+// The free page (FREE; otherwise the page in use) that has `rank` such pages
+// below it; groups[g] is the number of free pages in front of lane g's stretch.
+template <bool FREE>
 MI355_DEVICE uint32_t select_page(const BookPtrs& b, const uint32_t* groups, uint32_t lane_vecs, uint32_t rank) {
+  const uint32_t stretch = 128 * lane_vecs;
   uint32_t g = 0;  // the last stretch that starts at or in front of it
 #pragma unroll
-  for (uint32_t step = 512; step >= 1; step >>= 1)
-    if (groups[g + step] <= rank) g += step;
-  uint32_t r = rank - groups[g];
+  for (uint32_t step = 512; step >= 1; step >>= 1) {
+    const uint32_t front = FREE ? groups[g + step] : (g + step) * stretch - groups[g + step];
+    if (front <= rank && (FREE || (g + step) * stretch < b.num_pages)) g += step;
+  }
+  uint32_t r = rank - (FREE ? groups[g] : g * stretch - groups[g]);
   for (uint32_t v = g * lane_vecs; v < (g + 1) * lane_vecs; ++v) {
     const BitTile bits = load_bits_vec(b, v);
 #pragma unroll
     for (unsigned k = 0; k < 4; ++k) {
-      const uint32_t here = popcount32(bits.word[k]);
-      if (r < here) return 32 * (4 * v + k) + nth_bit(bits.word[k], r);
+      const uint32_t word = FREE ? bits.word[k] : existing_bits(b, ~bits.word[k], 4 * v + k);
+      const uint32_t here = popcount32(word);
+      if (r < here) return 32 * (4 * v + k) + nth_bit(word, r);
       r -= here;
     }
   }
-  return 0;  // not reached: the rank is below the number of free pages
+  return 0;  // not reached: the rank is below the number of such pages
 }
 
 // The page with rank nth goes to the entry whose share of the running sum of
@@ -324,7 +307,7 @@ MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
     if (granted && copies) {
       const uint32_t m = lds_add(&n_moves, 1);
       st_obj(a.moves.src + m, static_cast<int32_t>(tail));
-      st_obj(a.moves.dst + m, static_cast<int32_t>(select_page(b, groups, a.lane_vecs, carry + before)));
+      st_obj(a.moves.dst + m, static_cast<int32_t>(select_page<true>(b, groups, a.lane_vecs, carry + before)));
       st_obj(a.moves.valid + m, static_cast<int32_t>(fill));
       add_agent_i32(b.refs + tail, -1);
     }
@@ -336,7 +319,7 @@ MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
 #pragma unroll
         for (uint32_t step = 512; step >= 1; step >>= 1)
           if (start[e + step] <= t) e += step;
-        const uint32_t page = select_page(b, groups, a.lane_vecs, t);
+        const uint32_t page = select_page<true>(b, groups, a.lane_vecs, t);
         hand_out(b, page, t, start[e], who[e], slot_of[e]);
         tail = page;  // kept for below
       }
@@ -374,6 +357,26 @@ MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
   }
 }
 
+// A wave's 64 pages: each lane has the free bit of its page and how many free
+// pages are below it, of which pair_front are below all of them.
+struct PageLane {
+  uint32_t page, word, front;
+  bool exists, free;
+};
+
+MI355_DEVICE PageLane load_page_lane(const BookPtrs& b, uint32_t pair, uint32_t pair_front) {
+  const unsigned lane = thread_in_workgroup() & (kWave - 1);
+  const uint32_t index = 2 * pair + lane / 32;
+  PageLane p;
+  p.page = 64 * pair + lane;
+  p.exists = p.page < b.num_pages;
+  p.word = 32 * index < b.num_pages ? existing_bits(b, ld_u32<false>(b.bits + index), index) : 0;
+  const uint32_t low = lane_read(p.word, 0);
+  p.front = pair_front + (lane < 32 ? 0 : popcount32(low)) + popcount32(p.word & ((1u << (lane % 32)) - 1));
+  p.free = p.word >> (lane % 32) & 1;
+  return p;
+}
+
 // The second launch hands out what the first has left, a wave for 64 pages at
 // a time, a lane for each; the entry that a page goes to is found by bisection
 // of the running sum.
@@ -385,23 +388,19 @@ MI355_DEVICE void page_assign_body(const PageFinishArgs& a) {
     if (wanted == 0) return;
     const uint32_t front = ld_uniform_u32(a.work.pairs + pair);
     if (front >= wanted) return;  // and so it is for every later pair
-    const uint32_t index = 2 * pair + lane / 32;
-    uint32_t word = 0;
-    if (32 * index < b.num_pages) word = existing_bits(b, ld_u32<false>(b.bits + index), index);
-    const uint32_t low = lane_read(word, 0);
-    const uint32_t nth = front + (lane < 32 ? 0 : popcount32(low)) + popcount32(word & ((1u << (lane % 32)) - 1));
-    const bool taken = (word >> (lane % 32) & 1) && nth < wanted;
+    const PageLane p = load_page_lane(b, pair, front);
+    const bool taken = p.free && p.front < wanted;
     if (taken) {
       uint32_t e = 0;
 #pragma unroll
       for (uint32_t step = kMaxList / 2; step >= 1; step >>= 1)
-        if (e + step < a.n && ld_u32<false>(a.work.start + e + step) <= nth) e += step;
-      hand_out(b, 32 * index + lane % 32, nth, ld_u32<false>(a.work.start + e), ld_u32<false>(a.work.who + e),
+        if (e + step < a.n && ld_u32<false>(a.work.start + e + step) <= p.front) e += step;
+      hand_out(b, p.page, p.front, ld_u32<false>(a.work.start + e), ld_u32<false>(a.work.who + e),
                ld_u32<false>(a.work.slot + e));
     }
     const uint64_t gone = wave_ballot(taken);
     const uint32_t mine = lane < 32 ? static_cast<uint32_t>(gone) : static_cast<uint32_t>(gone >> 32);
-    if (lane % 32 == 0 && mine) st_u32(b.bits + index, word & ~mine);
+    if (lane % 32 == 0 && mine) st_u32(b.bits + p.page / 32, p.word & ~mine);
   }
 }
 
@@ -413,51 +412,105 @@ MI355_DEVICE void page_finish_body(const PageFinishArgs& a) {
     page_move_body<4, NTL, ST>(a.moves, global_wave(kMoveWaves) - a.assign_wgs * kMoveWaves);
 }
 
-// A sequence that holds its parent's pages.  A workgroup of 256 lanes for each
-// entry; the list is read by every one of them (it is short and in L2), so that
-// no entry depends on what another has already written: a child that an
-// earlier entry names too is left alone, and so is one whose parent is named
-// as a child.  Bound by the atomic additions.
-MI355_DEVICE void page_fork_body(const PageForkArgs& a) {
-  MI355_LDS uint32_t refused;
-  const BookPtrs& b = a.book;
-  const uint32_t t = thread_in_workgroup();
-  const uint32_t i = workgroup_index();
-  const uint32_t parent = static_cast<uint32_t>(ld_obj(a.parents + i));
-  const uint32_t child = static_cast<uint32_t>(ld_obj(a.children + i));
-  if (t == 0) refused = 0;
-  workgroup_barrier();
-  const bool in_range = parent < b.max_seqs && child < b.max_seqs;
-  if (in_range) {
-    bool bad = ld_obj(b.lengths + child) != 0;
-    for (uint32_t k = t; k < a.n; k += 256) {
-      const uint32_t c = static_cast<uint32_t>(ld_obj(a.children + k));
-      if (c == parent || (c == child && k < i)) bad = true;
-    }
-    if (bad) refused = 1;
+// Table entries j .. j + 3 of a sequence, those below `end`.
+struct FourPages {
+  uint32_t page[4];
+};
+
+MI355_DEVICE FourPages load_four(const int32_t* table, uint32_t j, uint32_t end) {
+  FourPages f;
+  if (end - j >= 4) {
+    const v4u v = ld_v4<false>(reinterpret_cast<const v4u_a4*>(table + j));
+    f.page[0] = v.x, f.page[1] = v.y, f.page[2] = v.z, f.page[3] = v.w;
+  } else {
+#pragma unroll
+    for (unsigned k = 0; k < 4; ++k) f.page[k] = j + k < end ? static_cast<uint32_t>(ld_obj(table + j + k)) : ~0u;
   }
-  workgroup_barrier();
-  const bool made = in_range && !refused;
-  if (made) {
-    const uint32_t tokens = ld_obj(b.lengths + parent);
-    uint32_t held = pages_held(tokens, b);
-    if (held > b.width) held = 0;  // not a length
-    const int32_t* from = b.tables + static_cast<uint64_t>(parent) * b.width;
-    int32_t* to = b.tables + static_cast<uint64_t>(child) * b.width;
-    for (uint32_t j = t; j < held; j += 256) {
-      const int32_t page = ld_obj(from + j);
-      st_obj(to + j, page);
-      if (static_cast<uint32_t>(page) < b.num_pages) add_agent_i32(b.refs + page, 1);
-    }
-    if (t == 0 && held) st_obj(b.lengths + child, static_cast<int32_t>(tokens));
-  }
-  if (t == 0 && a.granted) st_obj(a.granted + i, made ? 1 : 0);
+  return f;
 }
 
-// The end of a sequence, or of its tokens from `keep` on.  A workgroup of 256
-// lanes for each entry; lane 0 takes the sequence's tokens with an atomic
-// minimum, so that of two entries for one sequence each gives back what the
-// other has not.  Bound by the atomics.
+// A sequence that holds its parent's pages.  A workgroup for each entry.  Each
+// reads the whole list (it is short and in L2), and so decides
+// without what another may already have written: a child that an earlier entry
+// names too is left alone, and so is one whose parent is named as a child.
+//
+// The atomic additions are what it takes time for (20 of them in a nanosecond, whatever
+// their addresses), so the first entry that names a parent adds to its pages'
+// counts for all that do; an entry that is refused for its child's sake, which the
+// others cannot see, takes its own share off again.  1000 children of 90 parents,
+// 560 pages each: 27.5 us with an addition for each child and page.
+//
+// Where tables are long (a.made not null) an entry has a workgroup for each
+// 4096 pages, nobody writes a length, and another launch does.
+MI355_DEVICE void page_fork_body(const PageForkArgs& a) {
+  MI355_LDS uint32_t parent_named, again, first, holders;
+  const BookPtrs& b = a.book;
+  const uint32_t t = thread_in_workgroup();
+  const uint32_t i = workgroup_index() % a.n, chunk = workgroup_index() / a.n;
+  const uint32_t parent = static_cast<uint32_t>(ld_obj(a.parents + i));
+  const uint32_t child = static_cast<uint32_t>(ld_obj(a.children + i));
+  if (parent >= b.max_seqs || child >= b.max_seqs) {
+    if (t == 0 && chunk == 0) {
+      if (a.granted) st_obj(a.granted + i, 0);
+      if (a.made) st_u32(a.made + i, 0);
+    }
+    return;
+  }
+  if (t == 0) parent_named = 0, again = 0, first = ~0u, holders = 0;
+  const uint32_t tokens = ld_obj(b.lengths + parent);
+  // only the first entry that names the child writes it, after the barriers
+  const bool in_use = ld_obj(b.lengths + child) != 0;
+  uint32_t held = pages_held(tokens, b);
+  if (held > b.width) held = 0;  // not a length
+  if (chunk != 0 && chunk * kTableChunk >= held) return;
+  workgroup_barrier();
+  uint32_t mine = 0;
+  for (uint32_t k = t; k < a.n; k += a.wg_size) {
+    const uint32_t p = static_cast<uint32_t>(ld_obj(a.parents + k));
+    const uint32_t c = static_cast<uint32_t>(ld_obj(a.children + k));
+    if (c == parent) parent_named = 1;
+    if (c == child && k < i) again = 1;
+    if (p == parent && c < b.max_seqs) {
+      if (mine++ == 0) lds_min(&first, k);
+    }
+  }
+  if (mine) lds_add(&holders, mine);
+  workgroup_barrier();
+  const bool made = !parent_named && !again && !in_use;
+  if (!parent_named) {
+    const int32_t more = (first == i ? static_cast<int32_t>(holders) : 0) - (made ? 0 : 1);
+    const int32_t* from = b.tables + static_cast<uint64_t>(parent) * b.width;
+    int32_t* to = b.tables + static_cast<uint64_t>(child) * b.width;
+    uint32_t end = held;
+    if (a.made && end > (chunk + 1) * kTableChunk) end = (chunk + 1) * kTableChunk;
+    for (uint32_t j = chunk * kTableChunk + 4 * t; j < end; j += 4 * a.wg_size) {
+      const FourPages f = load_four(from, j, end);
+#pragma unroll
+      for (unsigned k = 0; k < 4; ++k) {
+        if (made && j + k < end) st_obj(to + j + k, static_cast<int32_t>(f.page[k]));
+        if (more && f.page[k] < b.num_pages) add_agent_i32(b.refs + f.page[k], more);
+      }
+    }
+  }
+  if (t != 0 || chunk != 0) return;
+  const uint32_t length = made && held ? tokens : 0;
+  if (a.made) st_u32(a.made + i, length);
+  else if (length) st_obj(b.lengths + child, static_cast<int32_t>(length));
+  if (a.granted) st_obj(a.granted + i, made ? 1 : 0);
+}
+
+MI355_DEVICE void page_fork_lengths_body(const PageForkArgs& a) {
+  const uint32_t i = workgroup_index() * 256 + thread_in_workgroup();
+  if (i >= a.n) return;
+  const uint32_t length = ld_u32<false>(a.made + i);
+  const uint32_t child = static_cast<uint32_t>(ld_obj(a.children + i));
+  if (length && child < a.book.max_seqs) st_obj(a.book.lengths + child, static_cast<int32_t>(length));
+}
+
+// The end of a sequence, or of its tokens from `keep` on.  A workgroup for each
+// entry; lane 0 takes the sequence's tokens with an atomic minimum, so that of
+// two entries for one sequence each gives back what the other has not.  Bound by
+// latency: entry, minimum, table, count, free bits.
 MI355_DEVICE void page_free_body(const PageFreeArgs& a) {
   MI355_LDS uint32_t before;
   const BookPtrs& b = a.book;
@@ -473,97 +526,185 @@ MI355_DEVICE void page_free_body(const PageFreeArgs& a) {
   uint32_t end = pages_held(was, b);
   if (end > b.width) end = b.width;
   const int32_t* table = b.tables + static_cast<uint64_t>(s) * b.width;
-  for (uint32_t j = pages_held(keep, b) + t; j < end; j += 256) {
-    const uint32_t page = static_cast<uint32_t>(ld_obj(table + j));
-    if (page >= b.num_pages) continue;
-    if (add_agent_i32(b.refs + page, -1) == 1) or_agent_u32(b.bits + page / 32, 1u << (page % 32));
+  for (uint32_t j = pages_held(keep, b) + 4 * t; j < end; j += 4 * a.wg_size) {
+    const FourPages f = load_four(table, j, end);
+    int32_t holders[4];
+#pragma unroll
+    for (unsigned k = 0; k < 4; ++k)
+      holders[k] = f.page[k] < b.num_pages ? add_agent_i32(b.refs + f.page[k], -1) : 0;
+    // pages that were handed out together often share a word
+    uint32_t word = ~0u, bits = 0;
+#pragma unroll
+    for (unsigned k = 0; k < 4; ++k) {
+      if (holders[k] != 1) continue;
+      if (f.page[k] / 32 != word) {
+        if (bits) or_agent_u32(b.bits + word, bits);
+        word = f.page[k] / 32, bits = 0;
+      }
+      bits |= 1u << (f.page[k] % 32);
+    }
+    if (bits) or_agent_u32(b.bits + word, bits);
   }
+}
+
+// The same for many pages, in two launches.  The device does some 20 atomics in
+// a nanosecond, so there is one for each page, whose result nobody waits for, and the
+// second launch makes the free bits from the counts and shortens the sequences
+// (306,000 pages of 850 sequences: 28 us with the free bits by atomics, 16 so).  A
+// workgroup for each entry and 4096 pages of its table; the first entry that
+// names a sequence acts for all that do, with the smallest keep of theirs.
+MI355_DEVICE void page_free_counts_body(const PageFreeArgs& a) {
+  MI355_LDS uint32_t again, least;
+  const BookPtrs& b = a.book;
+  const uint32_t t = thread_in_workgroup();
+  const uint32_t i = workgroup_index() % a.n, chunk = workgroup_index() / a.n;
+  const uint32_t s = static_cast<uint32_t>(ld_obj(a.seqs + i));
+  if (s >= b.max_seqs) return;
+  const int32_t tokens = ld_obj(b.lengths + s);
+  if (tokens <= 0) return;
+  uint32_t end = pages_held(tokens, b);
+  if (end > b.width) end = b.width;
+  if (chunk * kTableChunk >= end) return;
+  if (t == 0) again = 0, least = ~0u;
+  workgroup_barrier();
+  for (uint32_t k = t; k < a.n; k += a.wg_size) {
+    if (static_cast<uint32_t>(ld_obj(a.seqs + k)) != s) continue;
+    // a negative number is a large unsigned one
+    lds_min(&least, a.keep ? static_cast<uint32_t>(ld_obj(a.keep + k)) : 0);
+    if (k < i) again = 1;
+  }
+  workgroup_barrier();
+  if (again || least >= static_cast<uint32_t>(tokens)) return;
+  uint32_t j = pages_held(least, b);
+  if (j < chunk * kTableChunk) j = chunk * kTableChunk;
+  if (end > (chunk + 1) * kTableChunk) end = (chunk + 1) * kTableChunk;
+  const int32_t* table = b.tables + static_cast<uint64_t>(s) * b.width;
+  for (j += 4 * t; j < end; j += 4 * a.wg_size) {
+    const FourPages f = load_four(table, j, end);
+#pragma unroll
+    for (unsigned k = 0; k < 4; ++k)
+      if (f.page[k] < b.num_pages) add_agent_i32(b.refs + f.page[k], -1);
+  }
+}
+
+MI355_DEVICE void page_free_finish_body(const PageFreeArgs& a) {
+  const BookPtrs& b = a.book;
+  const unsigned lane = thread_in_workgroup() & (kWave - 1);
+  const uint32_t page = workgroup_index() * 256 + thread_in_workgroup();
+  const bool free = page < b.num_pages && ld_obj(b.refs + page) == 0;
+  const uint64_t all = wave_ballot(free);
+  const uint32_t word = lane < 32 ? static_cast<uint32_t>(all) : static_cast<uint32_t>(all >> 32);
+  if (lane % 32 == 0 && page < b.num_pages) st_u32(b.bits + page / 32, word);
+  const uint32_t i = page;
+  if (i >= a.n) return;
+  const uint32_t s = static_cast<uint32_t>(ld_obj(a.seqs + i));
+  const int32_t keep = a.keep ? ld_obj(a.keep + i) : 0;
+  if (s < b.max_seqs && keep >= 0) min_agent_i32(b.lengths + s, keep);
 }
 
 // Compaction.  With L pages in use, a page below L that is free is a hole and a
 // page from L on that is in use has to move; there are as many of the one as
-// of the other.  The i-th hole from below takes the i-th page from above, as far as the
-// caller's budget goes.  One workgroup of 1024 lanes makes the two lists from
-// the free bits (first how many pages are in use, then their ranks).
-MI355_DEVICE void page_compact_plan_body(const PageCompactArgs& a) {
-  MI355_LDS uint32_t scan_a[16], scan_b[16];
-  const BookPtrs& b = a.book;
-  const uint32_t t = thread_in_workgroup();
-  const uint32_t n_tiles = (b.num_pages + kTilePages - 1) / kTilePages;
-  uint32_t free_pages = 0;
-  for (uint32_t k = 0; k < n_tiles; ++k) {
-    uint32_t here;
-    block_scan_1024(count_bits(load_bits(b, k)), scan_a, &here);
-    free_pages += here;
-    workgroup_barrier();
-  }
-  const uint32_t live = b.num_pages - free_pages;
-  uint32_t holes = 0, movers = 0;
-  for (uint32_t k = 0; k < n_tiles; ++k) {
-    const BitTile bits = load_bits(b, k);
-    BitTile low, high;
-#pragma unroll
-    for (unsigned c = 0; c < 4; ++c) {
-      const uint32_t page = 32 * (k * kTileWords + 4 * t + c);
-      // pages of this word below `live`, and pages that exist
-      const uint32_t below = page >= live ? 0 : live - page >= 32 ? ~0u : (1u << (live - page)) - 1;
-      const uint32_t exist = page >= b.num_pages ? 0 : b.num_pages - page >= 32 ? ~0u : (1u << (b.num_pages - page)) - 1;
-      low.word[c] = bits.word[c] & below;
-      high.word[c] = ~bits.word[c] & ~below & exist;
-    }
-    uint32_t here;
-    uint32_t rank = holes + block_scan_1024(count_bits(low), scan_a, &here);
-    holes += here;
-#pragma unroll
-    for (unsigned c = 0; c < 4; ++c)
-      for (uint32_t m = low.word[c]; m; m &= m - 1, ++rank)
-        if (rank < a.max_moves)
-          st_obj(a.moves.dst + rank, static_cast<int32_t>(32 * (k * kTileWords + 4 * t + c) + lowest_bit(m)));
-    // every hole is below every page that moves: `holes` is final where one is met
-    rank = movers + block_scan_1024(count_bits(high), scan_b, &here);
-    movers += here;
-#pragma unroll
-    for (unsigned c = 0; c < 4; ++c)
-      for (uint32_t m = high.word[c]; m; m &= m - 1, ++rank) {
-        const uint32_t from_top = holes - 1 - rank;
-        if (from_top < a.max_moves)
-          st_obj(a.moves.src + from_top, static_cast<int32_t>(32 * (k * kTileWords + 4 * t + c) + lowest_bit(m)));
-      }
-    workgroup_barrier();
-  }
-  if (t == 0) {
-    const uint32_t n = holes < a.max_moves ? holes : a.max_moves;
-    st_obj(a.moves.count, PageMoveCount{n, 0, magic_divisor(n)});
-    st_obj(b.head, static_cast<int32_t>(n));
-  }
-}
+// of the other.  The i-th hole from below takes the i-th page from above, as far
+// as the caller's budget goes.
+//
+// Up to 1024 moves take two launches: one workgroup of 1024 lanes counts, and
+// finds by rank the hole and the page of each move, a lane for each; the second
+// moves the bytes, next to workgroups that rewrite the tables and the free bits.
+// Beyond, the first launch leaves the free pages in front of each two words of
+// the free bits and how many pages move, and one between the two, over the
+// whole device, finds for each hole the page that comes to it.
 
-// The counts and free bits of the pages that move, a lane for each.
-MI355_DEVICE void page_compact_apply_body(const PageCompactArgs& a) {
+// Move k, of page `from` to page `to`: the list, the counts, and what the caller wants to know.
+MI355_DEVICE void list_move(const PageCompactArgs& a, uint32_t k, uint32_t from, uint32_t to) {
   const BookPtrs& b = a.book;
-  const uint32_t n = ld_uniform_u32(&a.moves.count->n);
-  const uint32_t k = workgroup_index() * 256 + thread_in_workgroup();
-  if (k >= n) return;
-  const uint32_t from = ld_obj(a.moves.src + k), to = ld_obj(a.moves.dst + k);
+  st_obj(a.moves.src + k, static_cast<int32_t>(from));
+  st_obj(a.moves.dst + k, static_cast<int32_t>(to));
+  st_obj(a.moves.remap + from, static_cast<int32_t>(to));
   st_obj(b.refs + to, ld_obj(b.refs + from));
   st_obj(b.refs + from, 0);
-  or_agent_u32(b.bits + from / 32, 1u << (from % 32));
-  and_agent_u32(b.bits + to / 32, ~(1u << (to % 32)));
-  st_obj(a.moves.remap + from, static_cast<int32_t>(to));
   if (a.out) {
     st_obj(a.out + 2 * static_cast<uint64_t>(k), static_cast<int32_t>(from));
     st_obj(a.out + 2 * static_cast<uint64_t>(k) + 1, static_cast<int32_t>(to));
   }
 }
 
-// The tables, a workgroup of 256 lanes for each sequence.  The pages that moved
-// are the highest ones, so every held page from the lowest of them on has moved.
-MI355_DEVICE void page_compact_tables_body(const PageCompactArgs& a) {
+MI355_DEVICE void page_compact_plan_body(const PageCompactArgs& a) {
+  MI355_LDS uint32_t scan[16], groups[1024];
+  MI355_LDS uint32_t holes;
+  const BookPtrs& b = a.book;
+  const uint32_t t = thread_in_workgroup();
+  uint32_t mine = 0;
+  for (uint32_t k = 0; k < a.lane_vecs; ++k) mine += count_bits(load_bits_vec(b, t * a.lane_vecs + k));
+  if (t == 0) holes = 0;
+  uint32_t free_pages;
+  uint32_t front = block_scan_1024(mine, scan, &free_pages);
+  groups[t] = front;
+  const uint32_t live = b.num_pages - free_pages;
+  for (uint32_t k = 0; k < a.lane_vecs; ++k) {
+    const uint32_t v = t * a.lane_vecs + k;
+    if (128 * v >= b.num_pages) break;
+    const BitTile bits = load_bits_vec(b, v);
+    uint32_t at = front;
+#pragma unroll
+    for (unsigned c = 0; c < 4; ++c) {
+      const uint32_t page = 128 * v + 32 * c;
+      if (c % 2 == 0) st_u32(a.pairs + 2 * v + c / 2, at);
+      // the word that page L is in: the free pages below it are the holes
+      if (page <= live && live - page < 32) holes = at + popcount32(bits.word[c] & ((1u << (live - page)) - 1));
+      at += popcount32(bits.word[c]);
+    }
+    front = at;
+  }
+  workgroup_barrier();
+  const uint32_t n = holes < a.max_moves ? holes : a.max_moves;
+  if (t == 0) {
+    st_obj(a.moves.count, PageMoveCount{n, 0, magic_divisor(n)});
+    st_u32(a.live, live);
+    st_obj(b.head, static_cast<int32_t>(n));
+  }
+  if (a.max_moves <= kListedAtOnce && t < n)
+    list_move(a, t, select_page<false>(b, groups, a.lane_vecs, live - 1 - t), select_page<true>(b, groups, a.lane_vecs, t));
+}
+
+// The counts of the pages that move and where they go.
+MI355_DEVICE void page_compact_list_body(const PageCompactArgs& a) {
   const BookPtrs& b = a.book;
   const uint32_t n = ld_uniform_u32(&a.moves.count->n);
-  if (n == 0) return;
+  const uint32_t live = ld_uniform_u32(a.live);
+  for (uint32_t pair = static_cast<uint32_t>(global_wave(kMoveWaves)); pair < a.n_pairs; pair += a.pair_wgs * kMoveWaves) {
+    if (64 * pair >= live) return;
+    const uint32_t front = ld_uniform_u32(a.pairs + pair);
+    if (front >= n) return;  // the pages that move are all further down
+    const PageLane p = load_page_lane(b, pair, front);
+    const uint32_t k = p.front;
+    if (!p.free || p.page >= live || k >= n) continue;
+    // the page in use with live - 1 - k of them below it: the last pair with
+    // no more in front of it, and in it the bit
+    const uint32_t rank = live - 1 - k;
+    uint32_t lo = 0, hi = a.n_pairs;  // [lo, hi) holds it
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (64 * mid - ld_u32<false>(a.pairs + mid) <= rank) lo = mid; else hi = mid;
+    }
+    uint32_t r = rank - (64 * lo - ld_u32<false>(a.pairs + lo));
+    const uint32_t w0 = ~ld_u32<false>(b.bits + 2 * lo);
+    uint32_t from;
+    if (r < popcount32(w0)) {
+      from = 64 * lo + nth_bit(w0, r);
+    } else {
+      r -= popcount32(w0);
+      from = 64 * lo + 32 + nth_bit(~ld_u32<false>(b.bits + 2 * lo + 1), r);
+    }
+    if (from >= b.num_pages) from = p.page;  // not reached
+    list_move(a, k, from, p.page);
+  }
+}
+
+// The tables, a workgroup of 256 lanes for each sequence.  The pages that moved
+// are the highest ones, so every held page from the lowest of them on has moved.
+MI355_DEVICE void page_compact_tables_body(const PageCompactArgs& a, uint32_t n, uint32_t s) {
+  const BookPtrs& b = a.book;
   const uint32_t lowest = ld_uniform_u32(reinterpret_cast<const uint32_t*>(a.moves.src + n - 1));
-  const uint32_t s = workgroup_index();
   uint32_t held = pages_held(ld_obj(b.lengths + s), b);
   if (held > b.width) held = 0;
   int32_t* table = b.tables + static_cast<uint64_t>(s) * b.width;
@@ -571,6 +712,37 @@ MI355_DEVICE void page_compact_tables_body(const PageCompactArgs& a) {
     const uint32_t page = static_cast<uint32_t>(ld_obj(table + j));
     if (page >= lowest && page < b.num_pages) st_obj(table + j, ld_obj(a.moves.remap + page));
   }
+}
+
+// The free bits: the first n holes are taken, the last n pages in use are free.
+MI355_DEVICE void page_compact_bits_body(const PageCompactArgs& a, uint32_t n, uint32_t first_wave) {
+  const BookPtrs& b = a.book;
+  const unsigned lane = thread_in_workgroup() & (kWave - 1);
+  const uint32_t live = ld_uniform_u32(a.live);
+  for (uint32_t pair = first_wave; pair < a.n_pairs; pair += a.pair_wgs * kMoveWaves) {
+    const PageLane p = load_page_lane(b, pair, ld_uniform_u32(a.pairs + pair));
+    bool free = p.free;
+    if (p.exists && p.page < live && p.front < n) free = false;
+    // page - front pages in use are below it
+    if (p.exists && p.page >= live && live - (p.page - p.front) <= n) free = true;
+    const uint64_t all = wave_ballot(free);
+    const uint32_t word = lane < 32 ? static_cast<uint32_t>(all) : static_cast<uint32_t>(all >> 32);
+    if (lane % 32 == 0 && p.exists && word != p.word) st_u32(b.bits + p.page / 32, word);
+  }
+}
+
+template <bool NTL, int ST>
+MI355_DEVICE void page_compact_finish_body(const PageCompactFinishArgs& f) {
+  const PageCompactArgs& a = f.compact;
+  const uint32_t wg = workgroup_index();
+  const uint32_t n = ld_uniform_u32(&a.moves.count->n);
+  if (n == 0) return;
+  if (wg < a.pair_wgs)
+    page_compact_bits_body(a, n, static_cast<uint32_t>(global_wave(kMoveWaves)));
+  else if (wg < a.pair_wgs + a.book.max_seqs)
+    page_compact_tables_body(a, n, wg - a.pair_wgs);
+  else
+    page_move_body<1, NTL, ST>(f.moves, global_wave(kMoveWaves) - (a.pair_wgs + a.book.max_seqs) * static_cast<uint64_t>(kMoveWaves));
 }
 
 // An empty book: no tokens, no holders, every page free, no table entry.
@@ -611,11 +783,19 @@ MI355_FOR_EACH_PAGE_MOVE_KERNEL(MI355_DEFINE_PAGE_MOVE)
 MI355_FOR_EACH_PAGE_FINISH_KERNEL(MI355_DEFINE_PAGE_FINISH)
 
 MI355_KERNEL(1024) void mi355_pages_reserve(mi355::PageReserveArgs a) { mi355::page_reserve_body(a); }
-MI355_KERNEL(256) void mi355_pages_fork(mi355::PageForkArgs a) { mi355::page_fork_body(a); }
-MI355_KERNEL(256) void mi355_pages_free(mi355::PageFreeArgs a) { mi355::page_free_body(a); }
+MI355_KERNEL(1024) void mi355_pages_fork(mi355::PageForkArgs a) { mi355::page_fork_body(a); }
+MI355_KERNEL(256) void mi355_pages_fork_lengths(mi355::PageForkArgs a) { mi355::page_fork_lengths_body(a); }
+MI355_KERNEL(1024) void mi355_pages_free(mi355::PageFreeArgs a) { mi355::page_free_body(a); }
+MI355_KERNEL(1024) void mi355_pages_free_counts(mi355::PageFreeArgs a) { mi355::page_free_counts_body(a); }
+MI355_KERNEL(256) void mi355_pages_free_finish(mi355::PageFreeArgs a) { mi355::page_free_finish_body(a); }
 MI355_KERNEL(1024) void mi355_pages_compact_plan(mi355::PageCompactArgs a) { mi355::page_compact_plan_body(a); }
-MI355_KERNEL(256) void mi355_pages_compact_apply(mi355::PageCompactArgs a) { mi355::page_compact_apply_body(a); }
-MI355_KERNEL(256) void mi355_pages_compact_tables(mi355::PageCompactArgs a) { mi355::page_compact_tables_body(a); }
+MI355_KERNEL(256) void mi355_pages_compact_list(mi355::PageCompactArgs a) { mi355::page_compact_list_body(a); }
+//   mi355_pages_compact_finish_l<nt loads>_s<store policy>
+#define MI355_DEFINE_PAGE_COMPACT_FINISH(L, S)                                                       \
+  MI355_KERNEL(256) void mi355_pages_compact_finish_l##L##_s##S(mi355::PageCompactFinishArgs a) {    \
+    mi355::page_compact_finish_body<L != 0, S>(a);                                                   \
+  }
+MI355_FOR_EACH_PAGE_FINISH_KERNEL(MI355_DEFINE_PAGE_COMPACT_FINISH)
 MI355_KERNEL(256) void mi355_pages_reset(mi355::PageResetArgs a) { mi355::page_reset_body(a); }
 
 #endif  // MI355_BLIT_PAGES_KERNELS_H_

@@ -198,13 +198,13 @@ struct Cache {
   }
 
   static void run_moves(const Pool& to, const Pool& from, const int32_t* dst, const int32_t* src, const int32_t* valid,
-                        const PageMoveCount* count, uint64_t n, uint32_t route, uint32_t cus) {
-    PageMovePlan p = plan_page_moves(n, count ? 2 : 0, valid != nullptr, to.pieces, to.page_bytes, cus, route, 3);
+                        uint64_t n, uint32_t route, uint32_t cus) {
+    PageMovePlan p = plan_page_moves(n, 0, valid != nullptr, to.pieces, to.page_bytes, cus, route, 3);
     // the sizes here are small: the policies of large moves, and grids that stride
     if (p.store_policy == MI355_BLIT_STORE_CACHED && below(2)) p.nt_load = 1, p.store_policy = 1 + below(2);
     if (p.store_policy == MI355_BLIT_STORE_SYSTEM_WT) p.nt_load = below(2);
     if (below(2) && p.grid > 3) p.grid = 1 + below(p.grid);
-    const PageMoveArgs a{to.table[p.table], from.table[p.table], dst, src, valid, count,
+    const PageMoveArgs a{to.table[p.table], from.table[p.table], dst, src, valid, nullptr,
                          magic_divisor(static_cast<uint32_t>(n)), static_cast<uint32_t>(n), to.pieces[p.table],
                          to.c.pages, from.c.pages, to.c.rows, p.grid * kMoveWaves};
 #define TRY(U, L, S) \
@@ -230,6 +230,40 @@ struct Cache {
       case 0: return run(mi355_pages_reserve_finish_l0_s0, f, f.assign_wgs + p.grid, 256);
       case 1: return run(mi355_pages_reserve_finish_l1_s1, f, f.assign_wgs + p.grid, 256);
       default: return run(mi355_pages_reserve_finish_l1_s2, f, f.assign_wgs + p.grid, 256);
+    }
+  }
+
+  void run_fork(const Words& parents, const Words& children, int32_t* granted, uint32_t n) {
+    const uint32_t wg = below(2) ? table_wg_size(pool.c.width) : 128;
+    const bool split = below(2);
+    const PageForkArgs a{ptrs, parents.p.get(), children.p.get(), granted, split ? reserving.start : nullptr, n, wg};
+    run(mi355_pages_fork, a, split ? n * table_chunks(pool.c.width) : n, wg);
+    if (split) run(mi355_pages_fork_lengths, a, (n + 255) / 256, 256);
+  }
+
+  void run_free(const Words& seqs, const int32_t* keep, uint32_t n) {
+    const uint32_t wg = below(2) ? table_wg_size(pool.c.width) : 64;
+    const PageFreeArgs a{ptrs, seqs.p.get(), keep, n, wg};
+    if (below(2)) return run(mi355_pages_free, a, n, wg);
+    run(mi355_pages_free_counts, a, n * table_chunks(pool.c.width), wg);
+    run(mi355_pages_free_finish, a, ((pool.c.pages > n ? pool.c.pages : n) + 255) / 256, 256);
+  }
+
+  void run_compact(uint32_t most, int32_t* out) {
+    const uint32_t wgs = page_pair_wgs(pool.c.pages);
+    const PageCompactArgs a{ptrs, moves, reserving.pairs, reserving.wanted, out, most, reserve_lane_vecs(pool.c.pages),
+                            page_pairs(pool.c.pages), 1 + static_cast<uint32_t>(below(wgs))};
+    const PageMovePlan p = plan_page_moves(most, 2, false, pool.pieces, pool.page_bytes, 1 + below(3), 0, 3);
+    const PageCompactFinishArgs f{{pool.table[0], pool.table[0], moves.dst, moves.src, nullptr, moves.count,
+                                   magic_divisor(most), most, pool.pieces[0], pool.c.pages, pool.c.pages, pool.c.rows,
+                                   p.grid * kMoveWaves}, a};
+    const uint32_t grid = a.pair_wgs + pool.c.seqs + p.grid;
+    run(mi355_pages_compact_plan, a, 1, 1024);
+    if (most > kListedAtOnce) run(mi355_pages_compact_list, a, a.pair_wgs, 256);
+    switch (below(3)) {
+      case 0: return run(mi355_pages_compact_finish_l0_s0, f, grid, 256);
+      case 1: return run(mi355_pages_compact_finish_l1_s1, f, grid, 256);
+      default: return run(mi355_pages_compact_finish_l1_s2, f, grid, 256);
     }
   }
 
@@ -290,7 +324,7 @@ struct Cache {
     if (!n) return;
     Words p(parents), c(children), granted(List(n, 77));
     start(), reads(p), reads(c), writes(granted);
-    run(mi355_pages_fork, PageForkArgs{ptrs, p.p.get(), c.p.get(), granted.p.get(), n, 0}, n, 256);
+    run_fork(p, c, granted.p.get(), n);
     std::set<int32_t> named, all(children.begin(), children.end());
     for (uint32_t i = 0; i < n; ++i) {
       const int32_t a = parents[i], b = children[i];
@@ -313,7 +347,7 @@ struct Cache {
     if (!n) return;
     Words s(seqs), k(keep ? *keep : List());
     start(), reads(s), reads(k);
-    run(mi355_pages_free, PageFreeArgs{ptrs, s.p.get(), keep ? k.p.get() : nullptr, n, 0}, n, 256);
+    run_free(s, keep ? k.p.get() : nullptr, n);
     for (uint32_t i = 0; i < n; ++i) {
       const int32_t id = seqs[i], left = keep ? (*keep)[i] : 0;
       if (id < 0 || static_cast<uint32_t>(id) >= pool.c.seqs || left < 0 || left >= lengths[id]) continue;
@@ -328,11 +362,7 @@ struct Cache {
     if (!most) return;
     Words out(List(2 * static_cast<size_t>(most), -5));
     start(), writes(out);
-    const PageCompactArgs a{ptrs, moves, out.p.get(), most, 0};
-    run(mi355_pages_compact_plan, a, 1, 1024);
-    run(mi355_pages_compact_apply, a, (most + 255) / 256, 256);
-    run(mi355_pages_compact_tables, a, pool.c.seqs, 256);
-    run_moves(pool, pool, moves.dst, moves.src, nullptr, moves.count, most, 0, 1 + below(3));
+    run_compact(most, out.p.get());
     const auto before = pool.want;
     uint32_t k = 0, lo = 0, hi = pool.c.pages;
     for (;;) {
@@ -442,7 +472,7 @@ void random_copies() {
     a.allow(true), b.allow(true);
     for (const Words* w : {&ws, &wd, &wv}) g_check.allow_read(w->p.get(), w->n * 4);
     if (src.empty()) continue;
-    Cache::run_moves(to, a, wd.p.get(), ws.p.get(), cut ? wv.p.get() : nullptr, nullptr, src.size(), below(3), 1 + below(3));
+    Cache::run_moves(to, a, wd.p.get(), ws.p.get(), cut ? wv.p.get() : nullptr, src.size(), below(3), 1 + below(3));
     const auto before = a.want;
     for (size_t i = 0; i < src.size(); ++i) {
       if (static_cast<uint32_t>(src[i]) >= c.pages || static_cast<uint32_t>(dst[i]) >= c.pages) continue;
@@ -469,24 +499,20 @@ void random_words() {
     Words a(x), b(y), granted(List(n, 0)), out(List(c.pages + 2, 0));
     cache.start(), cache.reads(a), cache.reads(b), cache.writes(granted), cache.writes(out);
     cache.run_reserve(a, b, granted.p.get(), n);
-    Cache::run(mi355_pages_fork, PageForkArgs{cache.ptrs, a.p.get(), b.p.get(), granted.p.get(), n, 0}, n, 256);
-    Cache::run(mi355_pages_free, PageFreeArgs{cache.ptrs, a.p.get(), b.p.get(), n, 0}, n, 256);
+    cache.run_fork(a, b, granted.p.get(), n);
+    cache.run_free(a, b.p.get(), n);
     if (c.pages / 2) {
-      const PageCompactArgs p{cache.ptrs, cache.moves, out.p.get(), c.pages / 2, 0};
-      Cache::run(mi355_pages_compact_plan, p, 1, 1024);
-      Cache::run(mi355_pages_compact_apply, p, (c.pages / 2 + 255) / 256, 256);
-      Cache::run(mi355_pages_compact_tables, p, c.seqs, 256);
-      Cache::run_moves(cache.pool, cache.pool, cache.moves.dst, cache.moves.src, nullptr, cache.moves.count, c.pages / 2, 0, 2);
+      cache.run_compact(c.pages / 2, out.p.get());
     }
     ++g_calls;
   }
 }
 
-// More free pages than one tile of the free bits holds, and more than one
+// More pages than one vector of free bits for each lane covers, and more than one
 // round of entries that ask for them.
 void large_pool() {
   Config c;
-  c.rows = 1, c.seqs = 1500, c.width = 400, c.pages = kTilePages + 70001;
+  c.rows = 1, c.seqs = 1500, c.width = 400, c.pages = 131072 + 70001;
   c.planes.push_back({nullptr, 0, 1, 1});
   Cache cache;
   if (!cache.make(c)) return fail("a configuration was refused");
@@ -501,6 +527,22 @@ void large_pool() {
   cache.reserve(gone, List(gone.size(), 300));  // does not fit to its end
 }
 
+// Tables of several stretches of kTableChunk pages.
+void long_sequences() {
+  Config c;
+  c.rows = 3, c.seqs = 6, c.width = 3 * kTableChunk + 5, c.pages = 4 * kTableChunk;
+  c.planes.push_back({nullptr, 0, 1, 1});
+  Cache cache;
+  if (!cache.make(c)) return fail("a configuration was refused");
+  cache.reserve({0, 1}, {static_cast<int32_t>(3 * c.width - 1), static_cast<int32_t>(3 * kTableChunk)});
+  for (int turn = 0; turn < 6; ++turn) {
+    cache.fork({0, 1, 0, 9}, {2, 3, 2, 4});
+    const List keep = {static_cast<int32_t>(3 * kTableChunk + 7 * turn), 5, 100, 3};
+    cache.free_tokens({2, 3, 2, 5}, &keep);
+    cache.free_tokens({3, 2}, nullptr);
+  }
+}
+
 }  // namespace
 
 int main(int argc, char** argv) {
@@ -511,6 +553,7 @@ int main(int argc, char** argv) {
     g_state = 0x9E3779B97F4A7C15ull * (k + 1);
     g_at = "case " + std::to_string(k);
     if (k == 0) large_pool();
+    else if (k == 1) long_sequences();
     else if (k % 12 == 1) random_life(4, true);
     else if (k % 4 == 2) random_copies();
     else if (k % 4 == 3) random_words();
