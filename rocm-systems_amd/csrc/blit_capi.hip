@@ -864,6 +864,7 @@ struct mi355_blit_pages {
   uint64_t (*planes)[2] = nullptr;          // row_bytes and runs of each, to compare two pools by
   mi355::PagePlane* planes_dev[2] = {nullptr, nullptr};  // one allocation
   void* work_dev = nullptr;
+  bool even = true;                         // a page has as many bytes in every plane
   bool has_book = false;
   uint64_t book_words = 0;
   mi355::BookPtrs book{};
@@ -890,9 +891,11 @@ const PageCompactFinishVariant kPageCompactFinishVariants[] = {
 PageMoveArgs page_move_args(const mi355_blit_pages& to, const mi355_blit_pages& from, const PageMovePlan& p,
                             const int32_t* dst, const int32_t* src, const int32_t* valid, const PageMoveCount* count,
                             uint64_t n) {
+  // pieces of a page in each plane, where they are the same in all
+  const uint32_t even = to.even ? to.pieces[p.table] / to.n_planes : 0;
   return {to.planes_dev[p.table], from.planes_dev[p.table], dst, src, valid, count,
-          magic_divisor(static_cast<uint32_t>(n)), static_cast<uint32_t>(n), to.pieces[p.table],
-          to.num_pages, from.num_pages, to.rows, p.grid * kMoveWaves};
+          magic_divisor(static_cast<uint32_t>(n)), magic_divisor(even), static_cast<uint32_t>(n), to.pieces[p.table],
+          even, 0, to.num_pages, from.num_pages, to.rows, p.grid * kMoveWaves};
 }
 
 int launch_page_moves(const mi355_blit_pages& to, const mi355_blit_pages& from, const int32_t* dst, const int32_t* src,
@@ -944,7 +947,9 @@ int mi355_blit_pages_create(mi355_blit_t* h, const mi355_blit_pages_desc_t* desc
     for (uint32_t i = 0; i < desc->n_planes; ++i) {
       p->planes[i][0] = desc->planes[i].row_bytes;
       p->planes[i][1] = desc->planes[i].runs;
-      p->page_bytes += plane_page_bytes(desc->planes[i], desc->rows);
+      const uint64_t bytes = plane_page_bytes(desc->planes[i], desc->rows);
+      p->page_bytes += bytes;
+      if (bytes != plane_page_bytes(desc->planes[0], desc->rows)) p->even = false;
     }
     p->pieces[0] = pages_planes(*desc, kPieceUnrolls[0], table);
     p->pieces[1] = pages_planes(*desc, kPieceUnrolls[1], table + p->pieces[0]);

@@ -242,9 +242,7 @@ MI355_DEVICE uint32_t lds_or(uint32_t* p, uint32_t v) {
 }
 
 MI355_DEVICE unsigned popcount32(uint32_t v) { return __popc(v); }
-// Index of the lowest bit that is set; v is not 0.
-MI355_DEVICE unsigned lowest_bit(uint32_t v) { return static_cast<unsigned>(__ffs(static_cast<int>(v))) - 1; }
-
+MI355_DEVICE unsigned popcount64(uint64_t v) { return __popcll(v); }
 // Keeps the compiler from dropping a load whose value is not used.
 MI355_DEVICE void keep_alive(unsigned v) { asm volatile("" ::"v"(v)); }
 

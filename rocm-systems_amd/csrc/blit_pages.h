@@ -38,7 +38,8 @@ struct __attribute__((aligned(64))) PagePlane {
   uint32_t bytes;         // of a page in this plane
   uint32_t run_bytes;     // rows * row_bytes; 0 where the page is one run
   uint32_t row_bytes;
-  uint32_t pad[3];
+  uint32_t runs;
+  uint64_t magic_run;     // magic_divisor(run_bytes)
 };
 static_assert(sizeof(PagePlane) == 64, "one s_load_dwordx16");
 
@@ -59,8 +60,11 @@ struct PageMoveArgs {
   const int32_t* valid;        // rows of every run that are moved; null: all
   const PageMoveCount* count;  // the number of moves, at most n; null: n
   uint64_t magic_n;            // magic_divisor(n)
+  uint64_t magic_even;         // magic_divisor(even_pieces)
   uint32_t n;
-  uint32_t pieces;     // of a page, over all planes
+  uint32_t pieces;       // of a page, over all planes
+  uint32_t even_pieces;  // of a page in one plane, where all planes have the same number; 0 otherwise
+  uint32_t pad;
   uint32_t dst_pages;  // pages of each pool: others are not moved
   uint32_t src_pages;
   uint32_t rows;
@@ -279,7 +283,9 @@ inline uint32_t pages_planes(const mi355_blit_pages_desc_t& d, unsigned unroll, 
     r.magic_pieces = magic_divisor(r.pieces);
     r.first = first;
     r.run_bytes = p.runs > 1 ? d.rows * p.row_bytes : 0;
+    r.magic_run = magic_divisor(r.run_bytes);
     r.row_bytes = p.row_bytes;
+    r.runs = p.runs;
     for (uint32_t k = 0; out && k < r.pieces; ++k) out[first + k] = r;
     first += r.pieces;
   }

@@ -21,53 +21,41 @@ namespace mi355 {
 // the pages that are named, nothing else.
 // ---------------------------------------------------------------------------
 
-// A page of several runs of which only the first rows are moved: the bytes
-// whose place in their run is below `limit`.  A vector may lie across the end
-// of the rows or of a run; such a one goes byte by byte.  `offset` is the
-// piece's place in the page, `bytes` its length.
-template <bool NTL, int ST>
-MI355_DEVICE void move_cut_runs(uint8_t* d, const uint8_t* s, const PagePlane& g, unsigned offset, unsigned bytes,
-                                unsigned limit, unsigned lane) {
-  for (unsigned at = 16 * lane; at < bytes; at += 16 * kWave) {
-    const unsigned in_run = (offset + at) % g.run_bytes;
-    const unsigned left = bytes - at;
-    if (left >= 16 && in_run + 16 <= limit) {
-      st_v4_any<ST>(reinterpret_cast<uintptr_t>(d + at), ld_v4_any<NTL>(s + at));
-    } else if (in_run < limit || in_run + 16 > g.run_bytes) {
-      const unsigned n = left < 16 ? left : 16;
-      for (unsigned b = 0; b < n; ++b)
-        if ((offset + at + b) % g.run_bytes < limit) st_u8(d + at + b, ld_u8(s + at + b));
-    }
+// A page of several runs of which only the first rows are moved, `limit` bytes
+// of each run; dp and sp are the pages.  Where rows and runs are whole vectors,
+// the pieces are those of the moved bytes alone, one run's behind the other's, so that no
+// lane is idle and the last pieces are nobody's.
+template <int U, bool NTL, int ST>
+MI355_DEVICE void move_cut_runs(uint8_t* dp, const uint8_t* sp, const PagePlane& g, unsigned offset, unsigned limit,
+                                unsigned lane) {
+  const unsigned all = g.runs * limit;
+  const unsigned end = offset + piece_bytes(U) < all ? offset + piece_bytes(U) : all;
+  for (unsigned moved = offset + 16 * lane; moved < end; moved += 16 * kWave) {
+    const unsigned at = moved + moved / limit * (g.run_bytes - limit);
+    st_v4_any<ST>(reinterpret_cast<uintptr_t>(dp + at), ld_v4_any<NTL>(sp + at));
   }
 }
 
-template <int U, bool NTL, int ST>
-MI355_DEVICE void move_piece(uint8_t* d, const uint8_t* s, const PagePlane& g, unsigned offset, unsigned valid,
-                             unsigned rows, unsigned lane) {
-  unsigned bytes = g.bytes - offset < piece_bytes(U) ? g.bytes - offset : piece_bytes(U);
-  if (valid < rows) {
-    const unsigned limit = valid * g.row_bytes;
-    if (g.run_bytes) {
-      move_cut_runs<NTL, ST>(d, s, g, offset, bytes, limit, lane);
-      return;
+// The same for rows or runs that end inside a vector: the bytes of the piece at
+// `offset` whose place in their run is below `limit`, and a vector that lies across the end
+// of the rows or of a run byte by byte.
+template <bool NTL, int ST>
+MI355_DEVICE void move_odd_runs(uint8_t* d, const uint8_t* s, const PagePlane& g, unsigned offset, unsigned bytes,
+                                unsigned limit, unsigned lane) {
+  for (unsigned at = 16 * lane; at < bytes; at += 16 * kWave) {
+    const unsigned in_run = offset + at - div_magic(offset + at, g.magic_run) * g.run_bytes;
+    if (at + 16 <= bytes && in_run + 16 <= limit) {
+      st_v4_any<ST>(reinterpret_cast<uintptr_t>(d + at), ld_v4_any<NTL>(s + at));
+    } else if (in_run < limit || in_run + 16 > g.run_bytes) {
+      for (unsigned b = at; b < at + 16 && b < bytes; ++b)
+        if (offset + b - div_magic(offset + b, g.magic_run) * g.run_bytes < limit) st_u8(d + b, ld_u8(s + b));
     }
-    if (limit <= offset) return;
-    if (limit - offset < bytes) bytes = limit - offset;
   }
-  const unsigned vecs = bytes / 16;
-  v4u x[U];
-#pragma unroll
-  for (unsigned u = 0; u < U; ++u)
-    if (lane + u * kWave < vecs) x[u] = ld_v4_any<NTL>(s + 16 * (lane + u * kWave));
-#pragma unroll
-  for (unsigned u = 0; u < U; ++u)
-    if (lane + u * kWave < vecs) st_v4_any<ST>(reinterpret_cast<uintptr_t>(d + 16 * (lane + u * kWave)), x[u]);
-  const unsigned tail = bytes & 15;
-  if (lane < tail) st_u8(d + 16 * vecs + lane, ld_u8(s + 16 * vecs + lane));
 }
 
 template <int U, bool NTL, int ST>
 MI355_DEVICE void page_move_body(const PageMoveArgs& a, uint64_t first_wave) {
+  constexpr bool kCut = U == kPieceUnrolls[1];  // a.valid is not null
   const unsigned lane = thread_in_workgroup() & (kWave - 1);
   uint32_t n = a.n;
   uint64_t magic_n = a.magic_n;
@@ -79,22 +67,56 @@ MI355_DEVICE void page_move_body(const PageMoveArgs& a, uint64_t first_wave) {
   const uint64_t total = static_cast<uint64_t>(n) * a.pieces;
   for (uint64_t w = first_wave; w < total; w += a.n_waves) {
     const uint32_t item = static_cast<uint32_t>(w);
-    const uint32_t some_piece = div_magic(item, magic_n);
-    const PagePlane d = ld_uniform_plane(a.dst_planes + some_piece);
-    const uint32_t in_plane = item - n * d.first;
-    const uint32_t move = div_magic(in_plane, d.magic_pieces);
-    const uint32_t offset = (in_plane - move * d.pieces) * piece_bytes(U);
+    uint32_t some_piece = div_magic(item, magic_n);
+    uint32_t first = 0, pieces = a.even_pieces;
+    uint64_t magic_pieces = a.magic_even;
+    if (pieces) {
+      // the same number in all planes: the list can be read together with the planes
+      first = div_magic(some_piece, magic_pieces) * pieces;
+      some_piece = first;
+    } else {
+      const PagePlane p = ld_uniform_plane(a.dst_planes + some_piece);
+      first = p.first, pieces = p.pieces, magic_pieces = p.magic_pieces;
+    }
+    const uint32_t in_plane = item - n * first;
+    const uint32_t move = div_magic(in_plane, magic_pieces);
+    const uint32_t offset = (in_plane - move * pieces) * piece_bytes(U);
     const uint32_t to = ld_uniform_u32(reinterpret_cast<const uint32_t*>(a.dst + move));
     const uint32_t from = ld_uniform_u32(reinterpret_cast<const uint32_t*>(a.src + move));
+    const PagePlane d = ld_uniform_plane(a.dst_planes + some_piece);
+    const PagePlane s = ld_uniform_plane(a.src_planes + some_piece);
     uint32_t valid = a.rows;
-    if (a.valid) {
+    if constexpr (kCut) {
       const int32_t v = static_cast<int32_t>(ld_uniform_u32(reinterpret_cast<const uint32_t*>(a.valid + move)));
       if (v < static_cast<int32_t>(a.rows)) valid = v > 0 ? v : 0;
     }
     // a negative number is a large unsigned one
     if (to >= a.dst_pages || from >= a.src_pages || valid == 0) continue;
-    const PagePlane s = ld_uniform_plane(a.src_planes + some_piece);
-    move_piece<U, NTL, ST>(d.base + to * d.pitch + offset, s.base + from * s.pitch + offset, d, offset, valid, a.rows, lane);
+    uint8_t* dp = d.base + to * d.pitch + offset;
+    const uint8_t* sp = s.base + from * s.pitch + offset;
+    unsigned bytes = d.bytes - offset < piece_bytes(U) ? d.bytes - offset : piece_bytes(U);
+    if constexpr (kCut) {
+      if (valid < a.rows) {
+        const unsigned limit = valid * d.row_bytes;
+        if (d.run_bytes) {
+          if ((limit | d.run_bytes) % 16 == 0) move_cut_runs<U, NTL, ST>(dp - offset, sp - offset, d, offset, limit, lane);
+          else move_odd_runs<NTL, ST>(dp, sp, d, offset, bytes, limit, lane);
+          continue;
+        }
+        if (limit <= offset) continue;
+        if (limit - offset < bytes) bytes = limit - offset;
+      }
+    }
+    const unsigned vecs = bytes / 16;
+    v4u x[U];
+#pragma unroll
+    for (unsigned u = 0; u < U; ++u)
+      if (lane + u * kWave < vecs) x[u] = ld_v4_any<NTL>(sp + 16 * (lane + u * kWave));
+#pragma unroll
+    for (unsigned u = 0; u < U; ++u)
+      if (lane + u * kWave < vecs) st_v4_any<ST>(reinterpret_cast<uintptr_t>(dp + 16 * (lane + u * kWave)), x[u]);
+    const unsigned tail = bytes & 15;
+    if (lane < tail) st_u8(dp + 16 * vecs + lane, ld_u8(sp + 16 * vecs + lane));
   }
 }
 
@@ -218,9 +240,11 @@ MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
   const uint32_t t = thread_in_workgroup();
 
   // the free bits, a stretch for each lane
-  uint32_t mine = 0;
-  for (uint32_t k = 0; k < a.lane_vecs; ++k) mine += count_bits(load_bits_vec(b, t * a.lane_vecs + k));
-  for (uint32_t k = t; k < kMaxSeqs / 32; k += 1024) seen[k] = 0;
+  const BitTile kept = load_bits_vec(b, t * a.lane_vecs);
+  uint32_t mine = count_bits(kept);
+  for (uint32_t k = 1; k < a.lane_vecs; ++k) mine += count_bits(load_bits_vec(b, t * a.lane_vecs + k));
+  if (a.n > 1024)
+    for (uint32_t k = t; k < kMaxSeqs / 32; k += 1024) seen[k] = 0;
   if (t == 0) n_moves = 0, handed = 0;
   uint32_t free_pages;
   const uint32_t in_front = block_scan_1024(mine, scan_b, &free_pages);
@@ -248,14 +272,14 @@ MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
     bool again = false;
     if (named) {
       tokens = ld_obj(b.lengths + s);
-      again = seen[s / 32] >> (s % 32) & 1;
+      again = base && (seen[s / 32] >> (s % 32) & 1);
       slot = hash_slot(keys, s);
       lds_min(first + slot, t);
     }
     workgroup_barrier();
     if (named) {
       again = again || first[slot] != t;
-      lds_or(seen + s / 32, 1u << (s % 32));
+      if (a.n > 1024) lds_or(seen + s / 32, 1u << (s % 32));
     }
     // both below 2^31, so the sum is below 2^32
     const uint32_t old_pages = pages_held(tokens, b);
@@ -268,7 +292,8 @@ MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
       tail = ld_obj(b.tables + static_cast<uint64_t>(s) * b.width + old_pages - 1);
       if (tail < b.num_pages) {
         // an earlier round may have changed it
-        holders = ld_agent_u32(reinterpret_cast<const uint32_t*>(b.refs + tail));
+        holders = base ? ld_agent_u32(reinterpret_cast<const uint32_t*>(b.refs + tail))
+                       : static_cast<uint32_t>(ld_obj(b.refs + tail));
         shared = static_cast<int32_t>(holders) > 1;
       } else {
         ok = false;  // not a page
@@ -277,6 +302,7 @@ MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
     if (shared) any_shared = 1;
     workgroup_barrier();
     bool copies = shared;
+    uint32_t leavers = 0;  // not 0 in one of the askers of a page: how many of them copy it
     if (any_shared) {
       // With as many askers as holders, the last of them finds the page its own.
       for (uint32_t k = t; k < kSlots; k += 1024) keys[k] = kNoKey, first[k] = 0, asked[k] = 0;
@@ -287,7 +313,10 @@ MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
         lds_add(asked + slot, 1);
       }
       workgroup_barrier();
-      copies = shared && !(asked[slot] == holders && first[slot] == t);
+      if (shared && first[slot] == t) {
+        leavers = asked[slot];
+        if (leavers == holders) copies = false, --leavers;
+      }
     }
     uint32_t need = ok ? new_pages - old_pages + (copies ? 1 : 0) : 0;
     // more than the pool has is as good as one more: the sum over 1024 entries
@@ -301,31 +330,55 @@ MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
     start[t] = carry + before;
     who[t] = s | (copies ? 1u << 31 : 0);
     slot_of[t] = old_pages - (copies ? 1 : 0);
+    // the table of last pages is not needed any more (the sum has two barriers)
+    uint32_t *tail_of = keys, *fill_of = keys + 1024;
+    tail_of[t] = tail;
+    fill_of[t] = fill;
     workgroup_barrier();
     stopped = any_refused != 0;
     const uint32_t wanted = handed;  // up to here
-    if (granted && copies) {
-      const uint32_t m = lds_add(&n_moves, 1);
-      st_obj(a.moves.src + m, static_cast<int32_t>(tail));
-      st_obj(a.moves.dst + m, static_cast<int32_t>(select_page<true>(b, groups, a.lane_vecs, carry + before)));
-      st_obj(a.moves.valid + m, static_cast<int32_t>(fill));
-      add_agent_i32(b.refs + tail, -1);
+    const bool at_once = a.n <= 1024 && wanted <= 1024;
+    uint32_t page = 0, copy_of = ~0u;  // the entry whose last page is copied to `page`
+    if (at_once && t < wanted) {
+      uint32_t e = 0;  // the last entry that starts at or in front of the lane's page
+#pragma unroll
+      for (uint32_t step = 512; step >= 1; step >>= 1)
+        if (start[e + step] <= t) e += step;
+      page = select_page<true>(b, groups, a.lane_vecs, t);
+      hand_out(b, page, t, start[e], who[e], slot_of[e]);
+      if (t == start[e] && who[e] >> 31) copy_of = e;
+    } else if (!at_once && granted && copies) {
+      page = select_page<true>(b, groups, a.lane_vecs, carry + before);
+      copy_of = t;
     }
+    // a place in the list of moves, one addition for each wave
+    const uint64_t copying = wave_ballot(copy_of != ~0u);
+    uint32_t m = 0;
+    if (t % kWave == 0 && copying) m = lds_add(&n_moves, popcount64(copying));
+    m = lane_read(m, 0) + popcount64(copying & ((1ull << (t % kWave)) - 1));
+    if (copy_of != ~0u) {
+      st_obj(a.moves.src + m, static_cast<int32_t>(tail_of[copy_of]));
+      st_obj(a.moves.dst + m, static_cast<int32_t>(page));
+      st_obj(a.moves.valid + m, static_cast<int32_t>(fill_of[copy_of]));
+      if (stopped) add_agent_i32(b.refs + tail_of[copy_of], -1);
+    }
+    if (!stopped && leavers) st_obj(b.refs + tail, static_cast<int32_t>(holders - leavers));
     if (granted && more > 0) st_obj(b.lengths + s, static_cast<int32_t>(tokens + more));
     if (i < a.n && a.granted) st_obj(a.granted + i, granted ? 1 : 0);
-    if (a.n <= 1024 && wanted <= 1024) {
-      if (t < wanted) {
-        uint32_t e = 0;  // the last entry that starts at or in front of the lane's page
-#pragma unroll
-        for (uint32_t step = 512; step >= 1; step >>= 1)
-          if (start[e + step] <= t) e += step;
-        const uint32_t page = select_page<true>(b, groups, a.lane_vecs, t);
-        hand_out(b, page, t, start[e], who[e], slot_of[e]);
-        tail = page;  // kept for below
-      }
-      // every lane has read the bits it needs
+    if (at_once) {
+      // every lane has read the bits it needs; each takes the lowest ones out of its own stretch
       workgroup_barrier();
-      if (t < wanted) and_agent_u32(b.bits + tail / 32, ~(1u << (tail % 32)));
+      uint32_t left = in_front < wanted ? wanted - in_front : 0;
+      for (uint32_t v = t * a.lane_vecs; left && v < (t + 1) * a.lane_vecs; ++v) {
+        const BitTile bits = v == t * a.lane_vecs ? kept : load_bits_vec(b, v);
+#pragma unroll
+        for (unsigned k = 0; k < 4; ++k) {
+          const uint32_t here = popcount32(bits.word[k]);
+          if (left == 0 || here == 0) continue;
+          st_u32(b.bits + 4 * v + k, here <= left ? 0 : bits.word[k] >> nth_bit(bits.word[k], left) << nth_bit(bits.word[k], left));
+          left -= here <= left ? here : left;
+        }
+      }
       if (t == 0) handed = 0;
     } else {
       if (i < a.n) {
@@ -335,7 +388,7 @@ MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
       }
       carry = wanted;
       // the next round reads counts that this one wrote
-      wait_for_memory();
+      if (base + 1024 < a.n) wait_for_memory();
     }
     workgroup_barrier();
   }
@@ -344,7 +397,7 @@ MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
     for (uint32_t k = 0; k < a.lane_vecs; ++k) {
       const uint32_t v = t * a.lane_vecs + k;
       if (128 * v >= b.num_pages) break;
-      const BitTile bits = load_bits_vec(b, v);
+      const BitTile bits = k == 0 ? kept : load_bits_vec(b, v);
       st_u32(a.work.pairs + 2 * v, front);
       front += popcount32(bits.word[0]) + popcount32(bits.word[1]);
       st_u32(a.work.pairs + 2 * v + 1, front);

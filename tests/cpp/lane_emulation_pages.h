@@ -63,7 +63,7 @@ MI355_DEVICE uint64_t wave_ballot(bool v) {
 }
 
 MI355_DEVICE unsigned popcount32(uint32_t v) { return static_cast<unsigned>(__builtin_popcount(v)); }
-MI355_DEVICE unsigned lowest_bit(uint32_t v) { return static_cast<unsigned>(__builtin_ctz(v)); }
+MI355_DEVICE unsigned popcount64(uint64_t v) { return static_cast<unsigned>(__builtin_popcountll(v)); }
 
 }  // namespace mi355
 

@@ -68,6 +68,7 @@ struct Pool {
   PagePlane* table[2] = {nullptr, nullptr};
   uint32_t pieces[2] = {0, 0};
   uint64_t page_bytes = 0;
+  bool even = true;
   Pool() {}
   Pool(const Pool&) = delete;
   ~Pool() { std::free(table[0]), std::free(table[1]); }
@@ -82,6 +83,7 @@ struct Pool {
       c.planes[i].base = mem[i].p;
       want[i].assign(mem[i].p, mem[i].p + mem[i].n);
       page_bytes += page;
+      if (page != plane_page_bytes(c.planes[0], c.rows)) even = false;
     }
     mi355_blit_pages_desc_t d = desc(nullptr);
     uint64_t counted = 0;
@@ -197,6 +199,14 @@ struct Cache {
     if (g_m.errors) fail(g_m.first_error), g_m.errors = 0;
   }
 
+  static PageMoveArgs move_args(const Pool& to, const Pool& from, const PageMovePlan& p, const int32_t* dst,
+                                const int32_t* src, const int32_t* valid, const PageMoveCount* count, uint64_t n) {
+    const uint32_t even = to.even && below(2) ? to.pieces[p.table] / static_cast<uint32_t>(to.c.planes.size()) : 0;
+    return {to.table[p.table], from.table[p.table], dst, src, valid, count, magic_divisor(static_cast<uint32_t>(n)),
+            magic_divisor(even), static_cast<uint32_t>(n), to.pieces[p.table], even, 0, to.c.pages, from.c.pages,
+            to.c.rows, p.grid * kMoveWaves};
+  }
+
   static void run_moves(const Pool& to, const Pool& from, const int32_t* dst, const int32_t* src, const int32_t* valid,
                         uint64_t n, uint32_t route, uint32_t cus) {
     PageMovePlan p = plan_page_moves(n, 0, valid != nullptr, to.pieces, to.page_bytes, cus, route, 3);
@@ -204,9 +214,7 @@ struct Cache {
     if (p.store_policy == MI355_BLIT_STORE_CACHED && below(2)) p.nt_load = 1, p.store_policy = 1 + below(2);
     if (p.store_policy == MI355_BLIT_STORE_SYSTEM_WT) p.nt_load = below(2);
     if (below(2) && p.grid > 3) p.grid = 1 + below(p.grid);
-    const PageMoveArgs a{to.table[p.table], from.table[p.table], dst, src, valid, nullptr,
-                         magic_divisor(static_cast<uint32_t>(n)), static_cast<uint32_t>(n), to.pieces[p.table],
-                         to.c.pages, from.c.pages, to.c.rows, p.grid * kMoveWaves};
+    const PageMoveArgs a = move_args(to, from, p, dst, src, valid, nullptr, n);
 #define TRY(U, L, S) \
   if (kPieceUnrolls[p.table] == U && p.nt_load == L && p.store_policy == S) \
     return run(mi355_pages_move_u##U##_l##L##_s##S, a, p.grid, kMoveWaves * kWave);
@@ -222,10 +230,7 @@ struct Cache {
     const uint64_t copies = n < pool.c.pages ? n : pool.c.pages;
     const PageMovePlan p = plan_page_moves(copies, 2, true, pool.pieces, pool.page_bytes, 1 + below(3), 0, 3);
     const uint32_t n_pairs = (pool.c.pages + 63) / 64;
-    const PageFinishArgs f{{pool.table[1], pool.table[1], moves.dst, moves.src, moves.valid, moves.count,
-                            magic_divisor(static_cast<uint32_t>(copies)), static_cast<uint32_t>(copies), pool.pieces[1],
-                            pool.c.pages, pool.c.pages, pool.c.rows, p.grid * kMoveWaves},
-                           ptrs, reserving, n, n_pairs, 1 + static_cast<uint32_t>(below((n_pairs + 3) / 4)), 0};
+    const PageFinishArgs f{move_args(pool, pool, p, moves.dst, moves.src, moves.valid, moves.count, copies), ptrs, reserving, n, n_pairs, 1 + static_cast<uint32_t>(below((n_pairs + 3) / 4)), 0};
     switch (below(3)) {
       case 0: return run(mi355_pages_reserve_finish_l0_s0, f, f.assign_wgs + p.grid, 256);
       case 1: return run(mi355_pages_reserve_finish_l1_s1, f, f.assign_wgs + p.grid, 256);
@@ -254,9 +259,7 @@ struct Cache {
     const PageCompactArgs a{ptrs, moves, reserving.pairs, reserving.wanted, out, most, reserve_lane_vecs(pool.c.pages),
                             page_pairs(pool.c.pages), 1 + static_cast<uint32_t>(below(wgs))};
     const PageMovePlan p = plan_page_moves(most, 2, false, pool.pieces, pool.page_bytes, 1 + below(3), 0, 3);
-    const PageCompactFinishArgs f{{pool.table[0], pool.table[0], moves.dst, moves.src, nullptr, moves.count,
-                                   magic_divisor(most), most, pool.pieces[0], pool.c.pages, pool.c.pages, pool.c.rows,
-                                   p.grid * kMoveWaves}, a};
+    const PageCompactFinishArgs f{move_args(pool, pool, p, moves.dst, moves.src, nullptr, moves.count, most), a};
     const uint32_t grid = a.pair_wgs + pool.c.seqs + p.grid;
     run(mi355_pages_compact_plan, a, 1, 1024);
     if (most > kListedAtOnce) run(mi355_pages_compact_list, a, a.pair_wgs, 256);
@@ -409,6 +412,7 @@ Config some_config(bool wide) {
   for (size_t i = 0; i < n; ++i) {
     const uint32_t runs = below(2) ? 1 : static_cast<uint32_t>(between(2, 4));
     c.planes.push_back({nullptr, 0, static_cast<uint32_t>(between(1, wide ? 3 : below(4) ? 40 : 600)), runs});
+    if (below(2)) c.planes.back() = c.planes[0];
   }
   return c;
 }
