@@ -376,9 +376,10 @@ int mi355_blit_plan_rect_route(const mi355_pitched_ptr_t* dst, const mi355_dim3_
  * Everything a call reads or writes is in the GPU's memory (lists of sequences
  * and of pages, counts, what was granted), nothing is read back, and nothing is
  * allocated: a call is one to three kernel launches and may be recorded into a HIP graph.
- * Lists are arrays of int32_t; a number that is out of range (-1, say) is an
- * entry to pass over.  They are read when the commands run and have to stay as
- * they are until then.  Calls on one pool use its book and its work memory: those that may overlap --
+ * Lists are arrays of int32_t (an address that is no multiple of 4 ->
+ * INVALID_ARGUMENT); a number that is out of range (-1, say) is an entry to pass
+ * over.  They are read when the commands run, have to stay as they are until
+ * then, and may not share memory with what the call writes.  Calls on one pool use its book and its work memory: those that may overlap --
  * on different streams, or in graphs that are replayed at the same time, without an
  * ordering between them -- race and are the caller's to order, except
  * copies from and to pages that nothing else in flight writes.  stream is a
@@ -429,7 +430,8 @@ int mi355_blit_pages_book(uint32_t num_pages, uint32_t max_seqs, uint32_t max_pa
  * more than 2^31-1 bytes in one plane, sequences of more than 2^31-1 tokens,
  * 2^32 pieces of 1 KiB or more in the pool, or more than the limits above -> OUT_OF_RESOURCES.
  * The planes' and the book's memory stay the caller's and have to outlive the
- * object, and the object has to be destroyed before the handle. */
+ * object.  The object has to be destroyed before the handle: until then
+ * mi355_blit_destroy answers INVALID_ARGUMENT and leaves the handle as it is. */
 int mi355_blit_pages_create(mi355_blit_t* h, const mi355_blit_pages_desc_t* desc, mi355_blit_pages_t** out);
 
 /* Waits for the GPU, then frees the work memory.  Graphs that hold calls on the
@@ -449,7 +451,8 @@ int mi355_blit_pages_reset(mi355_blit_pages_t* p, void* stream);
  * mi355_blit_copy_route).  A sequence's row of the tables is such a list.
  * Lists that name a page as a destination twice, or both as a source and as a destination,
  * leave the bytes of that page undefined, as overlapping copies do.  NULL
- * list with n > 0, pools that differ -> INVALID_ARGUMENT; n pages of 2^32
+ * list with n > 0, pools that differ -> INVALID_ARGUMENT (the pools may have been made on two handles; `dst`'s
+ * is the one whose stream NULL means); n pages of 2^32
  * pieces of 1 KiB or more -> OUT_OF_RESOURCES; n == 0 -> SUCCESS without a launch.
  * No book is read or written. */
 int mi355_blit_pages_copy(mi355_blit_pages_t* dst, const int32_t* dst_pages, mi355_blit_pages_t* src,
@@ -492,7 +495,7 @@ int mi355_blit_pages_free(mi355_blit_pages_t* p, const int32_t* seqs, const int3
  * that has moved away are left.  The number of moves is left in the book's
  * head, and moves (NULL, or room for max_moves pairs) gets {from, to} of each,
  * the highest page first, for a caller that knows pages by number.
- * max_moves == 0 -> SUCCESS without a launch. */
+ * max_moves == 0 -> SUCCESS without a launch, the head left as it is. */
 int mi355_blit_pages_compact(mi355_blit_pages_t* p, uint32_t max_moves, int32_t* moves, void* stream);
 
 /* Decrements an HSA signal by 1 from the GPU once every command submitted

@@ -291,7 +291,8 @@ class Pages:
     """Owner of one mi355_blit_pages_t: the pages of a key/value cache, with a
     book (max_seqs, max_pages_per_seq and the device address of its buffer) or, for
     copies only, without.  planes: (base, pitch, row_bytes, runs) of each.  Methods
-    map 1:1 to the C ABI; lists are device addresses of int32."""
+    map 1:1 to the C ABI; lists are device addresses of int32.  Close it before the
+    Blit it was made with."""
 
     def __init__(self, blit, planes, num_pages, rows, max_seqs=0, max_pages_per_seq=0, book=None):
         self.lib = load()

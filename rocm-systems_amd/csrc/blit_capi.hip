@@ -142,6 +142,8 @@ struct mi355_blit {
   uint64_t* batch_seen = nullptr;
   size_t records_capacity = 0;
   size_t batch_capacity = 0;
+
+  unsigned pages_objects = 0;  // mi355_blit_pages that use this handle
 };
 
 namespace {
@@ -419,6 +421,7 @@ int mi355_blit_destroy(mi355_blit_t* h) {
   int rc = MI355_BLIT_SUCCESS;
   {
     std::lock_guard<std::mutex> g(h->lock);
+    if (h->pages_objects) return MI355_BLIT_ERROR_INVALID_ARGUMENT;
     DeviceScope scope(h->device);
     // every command, on whichever stream it went, is behind a marker
     if (h->ledger[0].done && ledger_mark(h) != MI355_BLIT_SUCCESS) rc = MI355_BLIT_ERROR;
@@ -912,9 +915,13 @@ int launch_page_moves(const mi355_blit_pages& to, const mi355_blit_pages& from, 
   return MI355_BLIT_SUCCESS;
 }
 
+// Whether a list of numbers is where the kernels can read it (null: no list).
+bool aligned_list(const void* list) { return (reinterpret_cast<uintptr_t>(list) & 3) == 0; }
+
 // What every call on a book checks before it looks at its lists.
-int check_book_call(const mi355_blit_pages* p, bool lists, size_t n) {
-  if (!p || !p->has_book || (n && !lists)) return MI355_BLIT_ERROR_INVALID_ARGUMENT;
+int check_book_call(const mi355_blit_pages* p, size_t n, const void* list, const void* other, const void* third) {
+  if (!p || !p->has_book || (n && !list)) return MI355_BLIT_ERROR_INVALID_ARGUMENT;
+  if (!aligned_list(list) || !aligned_list(other) || !aligned_list(third)) return MI355_BLIT_ERROR_INVALID_ARGUMENT;
   if (n > MI355_BLIT_PAGES_MAX_LIST) return MI355_BLIT_ERROR_OUT_OF_RESOURCES;
   return MI355_BLIT_SUCCESS;
 }
@@ -975,6 +982,7 @@ int mi355_blit_pages_create(mi355_blit_t* h, const mi355_blit_pages_desc_t* desc
   }
   std::free(table);
   if (rc == MI355_BLIT_SUCCESS && e == hipSuccess) {
+    ++h->pages_objects;
     *out = p;
     return MI355_BLIT_SUCCESS;
   }
@@ -984,6 +992,7 @@ int mi355_blit_pages_create(mi355_blit_t* h, const mi355_blit_pages_desc_t* desc
     std::free(p->planes);
     delete p;
   }
+  (void)hipGetLastError();  // reported here, not by the next call
   return rc != MI355_BLIT_SUCCESS ? rc : status_of(e);
 }
 
@@ -997,6 +1006,7 @@ int mi355_blit_pages_destroy(mi355_blit_pages_t* p) {
     BLIT_HIP(hipDeviceSynchronize());
     (void)hipFree(p->planes_dev[0]);
     if (p->work_dev) (void)hipFree(p->work_dev);
+    --p->h->pages_objects;
   }
   std::free(p->planes);
   delete p;
@@ -1020,6 +1030,8 @@ int mi355_blit_pages_copy(mi355_blit_pages_t* dst, const int32_t* dst_pages, mi3
                           void* stream) {
   if (!dst || !src || route > MI355_BLIT_ROUTE_DEVICE_TO_HOST || (n && (!dst_pages || !src_pages)))
     return MI355_BLIT_ERROR_INVALID_ARGUMENT;
+  if (!aligned_list(dst_pages) || !aligned_list(src_pages) || !aligned_list(valid_rows))
+    return MI355_BLIT_ERROR_INVALID_ARGUMENT;
   if (dst != src && (dst->h->device != src->h->device || dst->rows != src->rows || dst->n_planes != src->n_planes ||
                      std::memcmp(dst->planes, src->planes, dst->n_planes * sizeof(*dst->planes)) != 0))
     return MI355_BLIT_ERROR_INVALID_ARGUMENT;
@@ -1034,7 +1046,7 @@ int mi355_blit_pages_copy(mi355_blit_pages_t* dst, const int32_t* dst_pages, mi3
 
 int mi355_blit_pages_reserve(mi355_blit_pages_t* p, const int32_t* seqs, const int32_t* more, size_t n,
                              int32_t* granted, void* stream) {
-  const int rc = check_book_call(p, seqs && more, n);
+  const int rc = check_book_call(p, n, more ? seqs : nullptr, more, granted);
   if (rc != MI355_BLIT_SUCCESS || n == 0) return rc;
   std::lock_guard<std::mutex> g(p->h->lock);
   DeviceScope scope(p->h->device);
@@ -1061,7 +1073,7 @@ int mi355_blit_pages_reserve(mi355_blit_pages_t* p, const int32_t* seqs, const i
 
 int mi355_blit_pages_fork(mi355_blit_pages_t* p, const int32_t* parents, const int32_t* children, size_t n,
                           int32_t* granted, void* stream) {
-  const int rc = check_book_call(p, parents && children, n);
+  const int rc = check_book_call(p, n, children ? parents : nullptr, children, granted);
   if (rc != MI355_BLIT_SUCCESS || n == 0) return rc;
   std::lock_guard<std::mutex> g(p->h->lock);
   DeviceScope scope(p->h->device);
@@ -1070,7 +1082,8 @@ int mi355_blit_pages_fork(mi355_blit_pages_t* p, const int32_t* parents, const i
   const uint32_t wg = table_wg_size(p->book.width);
   const bool split = p->book.width > kSplitWidth;
   const uint32_t count = static_cast<uint32_t>(n);
-  const PageForkArgs a{p->book, parents, children, granted, split ? p->reserve.start : nullptr, count, wg};
+  const PageForkArgs a{p->book, parents, children, granted, split ? p->reserve.start : nullptr, count, wg,
+                       table_chunk(p->book.width), 0};
   hipLaunchKernelGGL(mi355_pages_fork, dim3(split ? count * table_chunks(p->book.width) : count), dim3(wg), 0, s, a);
   if (split) hipLaunchKernelGGL(mi355_pages_fork_lengths, dim3((count + 255) / 256), dim3(256), 0, s, a);
   BLIT_HIP(hipGetLastError());
@@ -1078,7 +1091,7 @@ int mi355_blit_pages_fork(mi355_blit_pages_t* p, const int32_t* parents, const i
 }
 
 int mi355_blit_pages_free(mi355_blit_pages_t* p, const int32_t* seqs, const int32_t* keep, size_t n, void* stream) {
-  const int rc = check_book_call(p, seqs != nullptr, n);
+  const int rc = check_book_call(p, n, seqs, keep, nullptr);
   if (rc != MI355_BLIT_SUCCESS || n == 0) return rc;
   std::lock_guard<std::mutex> g(p->h->lock);
   DeviceScope scope(p->h->device);
@@ -1086,7 +1099,7 @@ int mi355_blit_pages_free(mi355_blit_pages_t* p, const int32_t* seqs, const int3
   hipStream_t s = stream ? static_cast<hipStream_t>(stream) : p->h->stream;
   const uint32_t wg = table_wg_size(p->book.width);
   const uint32_t count = static_cast<uint32_t>(n);
-  const PageFreeArgs a{p->book, seqs, keep, count, wg};
+  const PageFreeArgs a{p->book, seqs, keep, count, wg, table_chunk(p->book.width), 0};
   if (n * p->book.width < kFreeByCounts && p->book.width <= kSplitWidth) {
     hipLaunchKernelGGL(mi355_pages_free, dim3(count), dim3(wg), 0, s, a);
   } else {
@@ -1099,7 +1112,7 @@ int mi355_blit_pages_free(mi355_blit_pages_t* p, const int32_t* seqs, const int3
 }
 
 int mi355_blit_pages_compact(mi355_blit_pages_t* p, uint32_t max_moves, int32_t* moves, void* stream) {
-  if (!p || !p->has_book) return MI355_BLIT_ERROR_INVALID_ARGUMENT;
+  if (!p || !p->has_book || !aligned_list(moves)) return MI355_BLIT_ERROR_INVALID_ARGUMENT;
   // a hole for each page that moves
   const uint32_t most = max_moves < p->num_pages / 2 ? max_moves : p->num_pages / 2;
   if (most == 0) return MI355_BLIT_SUCCESS;

@@ -135,6 +135,8 @@ struct PageForkArgs {
   uint32_t* made;    // not null: the children's lengths for the second launch
   uint32_t n;
   uint32_t wg_size;
+  uint32_t chunk;    // pages of a table that one workgroup goes through
+  uint32_t pad;
 };
 
 struct PageFreeArgs {
@@ -143,6 +145,8 @@ struct PageFreeArgs {
   const int32_t* keep;  // null: 0
   uint32_t n;
   uint32_t wg_size;
+  uint32_t chunk;       // as in PageForkArgs
+  uint32_t pad;
 };
 
 struct PageCompactArgs {
@@ -295,11 +299,17 @@ inline uint32_t pages_planes(const mi355_blit_pages_desc_t& d, unsigned unroll, 
 // Lanes for each entry of a call that goes through tables of `width` pages, four
 // at a time.
 inline uint32_t table_wg_size(uint32_t width) { return width <= 1024 ? 256 : 1024; }
-// Pages of a table that one workgroup goes through where an entry has several,
-// and the width from which on it has.
+// Pages of a table that one workgroup goes through where an entry has several
+// (64 of them at most, so that a grid for the longest list has a size), and the
+// width from which on it has.
 constexpr uint32_t kTableChunk = 4096;
 constexpr uint32_t kSplitWidth = 2 * kTableChunk;
-inline uint32_t table_chunks(uint32_t width) { return (width + kTableChunk - 1) / kTableChunk; }
+inline uint32_t table_chunk(uint32_t width) {
+  const uint32_t share = (width / 64 + 4) / 4 * 4;
+  return share > kTableChunk ? share : kTableChunk;
+}
+inline uint32_t table_chunks(uint32_t width) { return (width + table_chunk(width) - 1) / table_chunk(width); }
+static_assert(64ull * kMaxList * 1024 <= kMaxGridWorkItems, "work-items of a grid are counted in 31 bits");
 
 // From so many pages that a list can free on, the free bits are made from the
 // counts: 256 sequences of 375 pages (width 512) 14.4 us with an atomic for each

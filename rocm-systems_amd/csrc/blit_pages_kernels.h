@@ -494,7 +494,7 @@ MI355_DEVICE FourPages load_four(const int32_t* table, uint32_t j, uint32_t end)
 // 560 pages each: 27.5 us with an addition for each child and page.
 //
 // Where tables are long (a.made not null) an entry has a workgroup for each
-// 4096 pages, nobody writes a length, and another launch does.
+// a.chunk pages, nobody writes a length, and another launch does.
 MI355_DEVICE void page_fork_body(const PageForkArgs& a) {
   MI355_LDS uint32_t parent_named, again, first, holders;
   const BookPtrs& b = a.book;
@@ -515,7 +515,7 @@ MI355_DEVICE void page_fork_body(const PageForkArgs& a) {
   const bool in_use = ld_obj(b.lengths + child) != 0;
   uint32_t held = pages_held(tokens, b);
   if (held > b.width) held = 0;  // not a length
-  if (chunk != 0 && chunk * kTableChunk >= held) return;
+  if (chunk != 0 && chunk * a.chunk >= held) return;
   workgroup_barrier();
   uint32_t mine = 0;
   for (uint32_t k = t; k < a.n; k += a.wg_size) {
@@ -535,8 +535,8 @@ MI355_DEVICE void page_fork_body(const PageForkArgs& a) {
     const int32_t* from = b.tables + static_cast<uint64_t>(parent) * b.width;
     int32_t* to = b.tables + static_cast<uint64_t>(child) * b.width;
     uint32_t end = held;
-    if (a.made && end > (chunk + 1) * kTableChunk) end = (chunk + 1) * kTableChunk;
-    for (uint32_t j = chunk * kTableChunk + 4 * t; j < end; j += 4 * a.wg_size) {
+    if (a.made && end > (chunk + 1) * a.chunk) end = (chunk + 1) * a.chunk;
+    for (uint32_t j = chunk * a.chunk + 4 * t; j < end; j += 4 * a.wg_size) {
       const FourPages f = load_four(from, j, end);
 #pragma unroll
       for (unsigned k = 0; k < 4; ++k) {
@@ -604,7 +604,7 @@ MI355_DEVICE void page_free_body(const PageFreeArgs& a) {
 // a nanosecond, so there is one for each page, whose result nobody waits for, and the
 // second launch makes the free bits from the counts and shortens the sequences
 // (306,000 pages of 850 sequences: 28 us with the free bits by atomics, 16 so).  A
-// workgroup for each entry and 4096 pages of its table; the first entry that
+// workgroup for each entry and a.chunk pages of its table; the first entry that
 // names a sequence acts for all that do, with the smallest keep of theirs.
 MI355_DEVICE void page_free_counts_body(const PageFreeArgs& a) {
   MI355_LDS uint32_t again, least;
@@ -617,7 +617,7 @@ MI355_DEVICE void page_free_counts_body(const PageFreeArgs& a) {
   if (tokens <= 0) return;
   uint32_t end = pages_held(tokens, b);
   if (end > b.width) end = b.width;
-  if (chunk * kTableChunk >= end) return;
+  if (chunk * a.chunk >= end) return;
   if (t == 0) again = 0, least = ~0u;
   workgroup_barrier();
   for (uint32_t k = t; k < a.n; k += a.wg_size) {
@@ -629,8 +629,8 @@ MI355_DEVICE void page_free_counts_body(const PageFreeArgs& a) {
   workgroup_barrier();
   if (again || least >= static_cast<uint32_t>(tokens)) return;
   uint32_t j = pages_held(least, b);
-  if (j < chunk * kTableChunk) j = chunk * kTableChunk;
-  if (end > (chunk + 1) * kTableChunk) end = (chunk + 1) * kTableChunk;
+  if (j < chunk * a.chunk) j = chunk * a.chunk;
+  if (end > (chunk + 1) * a.chunk) end = (chunk + 1) * a.chunk;
   const int32_t* table = b.tables + static_cast<uint64_t>(s) * b.width;
   for (j += 4 * t; j < end; j += 4 * a.wg_size) {
     const FourPages f = load_four(table, j, end);

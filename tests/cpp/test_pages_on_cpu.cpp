@@ -241,14 +241,15 @@ struct Cache {
   void run_fork(const Words& parents, const Words& children, int32_t* granted, uint32_t n) {
     const uint32_t wg = below(2) ? table_wg_size(pool.c.width) : 128;
     const bool split = below(2);
-    const PageForkArgs a{ptrs, parents.p.get(), children.p.get(), granted, split ? reserving.start : nullptr, n, wg};
+    const PageForkArgs a{ptrs, parents.p.get(), children.p.get(), granted, split ? reserving.start : nullptr, n, wg,
+                         table_chunk(pool.c.width), 0};
     run(mi355_pages_fork, a, split ? n * table_chunks(pool.c.width) : n, wg);
     if (split) run(mi355_pages_fork_lengths, a, (n + 255) / 256, 256);
   }
 
   void run_free(const Words& seqs, const int32_t* keep, uint32_t n) {
     const uint32_t wg = below(2) ? table_wg_size(pool.c.width) : 64;
-    const PageFreeArgs a{ptrs, seqs.p.get(), keep, n, wg};
+    const PageFreeArgs a{ptrs, seqs.p.get(), keep, n, wg, table_chunk(pool.c.width), 0};
     if (below(2)) return run(mi355_pages_free, a, n, wg);
     run(mi355_pages_free_counts, a, n * table_chunks(pool.c.width), wg);
     run(mi355_pages_free_finish, a, ((pool.c.pages > n ? pool.c.pages : n) + 255) / 256, 256);

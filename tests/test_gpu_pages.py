@@ -398,6 +398,22 @@ def test_a_list_of_the_longest_kind(torch_cuda, capi, engine, rand):
         c.close()
 
 
+def test_holders_of_a_page_in_different_rounds_of_a_list(torch_cuda, capi, engine, rand):
+    """A list is taken 1024 entries at a time: what an earlier round has left of a page's
+    holders is what a later one finds."""
+    n = 2600
+    c = Cache(torch_cuda, capi, engine, rand, 12000, 16, 3 * n, 2, [(4, 1, 0, 0)])
+    try:
+        c.reserve(list(range(n)), [1 + i % 20 for i in range(n)])
+        c.fork(list(range(n)), list(range(n, 2 * n)))
+        c.fork(list(range(0, n, 3)), list(range(2 * n, 2 * n + len(range(0, n, 3)))))
+        # parents first, then the children in another order: the last to come keeps the page
+        c.reserve(list(range(n)) + list(range(2 * n - 1, n - 1, -1)) + list(range(2 * n, 3 * n))[:900], [1] * (2 * n + 900))
+        c.free(list(range(0, 3 * n, 2)) + list(range(0, 300)), [i % 7 for i in range(len(range(0, 3 * n, 2)) + 300)])
+    finally:
+        c.close()
+
+
 def test_a_large_pool(torch_cuda, capi, engine, rand):
     """More pages than one tile of the free bits covers, sequences of tens of thousands."""
     pages = 131072 + 70001
@@ -541,6 +557,18 @@ def test_refusals(torch_cuda, capi, engine, rand):
         assert p.fork(lists, lists, too_many) == res and p.fork(None, None, 0) == capi.SUCCESS
         assert p.free(None, 1) == inv and p.free(lists, too_many) == res and p.free(None, 0) == capi.SUCCESS
         assert p.compact(0) == capi.SUCCESS
+        # lists at addresses that are no multiple of 4
+        assert pool.copy(lists + 2, lists, 1) == inv and pool.copy(lists, lists + 1, 1) == inv
+        assert pool.copy(lists, lists, 1, valid=lists + 3) == inv
+        assert p.reserve(lists + 1, lists, 1) == inv and p.reserve(lists, lists + 2, 1) == inv
+        assert p.reserve(lists, lists, 1, granted=lists + 2) == inv
+        assert p.fork(lists + 2, lists, 1) == inv and p.fork(lists, lists + 2, 1) == inv
+        assert p.fork(lists, lists, 1, granted=lists + 1) == inv
+        assert p.free(lists + 2, 1) == inv and p.free(lists, 1, keep=lists + 2) == inv
+        assert p.compact(1, moves=lists + 2) == inv
+        # the handle stays while something uses it
+        assert capi.load().mi355_blit_destroy(engine.handle) == inv
+        assert engine.synchronize() == capi.SUCCESS
     torch.cuda.synchronize()
     assert int(buf.sum()) == 0 and int(book.sum()) == 0
 
