@@ -379,12 +379,15 @@ int mi355_blit_plan_rect_route(const mi355_pitched_ptr_t* dst, const mi355_dim3_
  * Lists are arrays of int32_t (an address that is no multiple of 4 ->
  * INVALID_ARGUMENT); a number that is out of range (-1, say) is an entry to pass
  * over.  They are read when the commands run, have to stay as they are until
- * then, and may not share memory with what the call writes.  Calls on one pool use its book and its work memory: those that may overlap --
- * on different streams, or in graphs that are replayed at the same time, without an
- * ordering between them -- race and are the caller's to order, except
- * copies from and to pages that nothing else in flight writes.  stream is a
- * hipStream_t, or NULL for the handle's own.  Like the allocation-free batch
- * these commands are not entered in the pending-bytes ledger. */
+ * then, and may not share memory with what the call writes.  Calls on one book
+ * use the object's work memory: those that may overlap -- on different streams,
+ * or in graphs that are replayed at the same time, without an ordering between
+ * them -- race and are the caller's to order.  Copies use none, and race only
+ * with what writes the pages that they name.  stream is a hipStream_t, or NULL
+ * for the handle's own (which is not ordered with the default stream).  Like the
+ * allocation-free batch these commands are not entered in the pending-bytes
+ * ledger, and neither mi355_blit_set_tuning nor mi355_blit_last_launch_info
+ * knows of them. */
 typedef struct mi355_blit_pages mi355_blit_pages_t;
 
 /* Sequences that one call can name, sequences and pages that a book can have. */
@@ -449,12 +452,13 @@ int mi355_blit_pages_reset(mi355_blit_pages_t* p, void* stream);
  * each plane (bases and pitches may differ), on the same GPU; either may be host memory that the GPU can
  * access, with the route that says so (MI355_BLIT_ROUTE_*, as in
  * mi355_blit_copy_route).  A sequence's row of the tables is such a list.
- * Lists that name a page as a destination twice, or both as a source and as a destination,
- * leave the bytes of that page undefined, as overlapping copies do.  NULL
- * list with n > 0, pools that differ -> INVALID_ARGUMENT (the pools may have been made on two handles; `dst`'s
- * is the one whose stream NULL means); n pages of 2^32
- * pieces of 1 KiB or more -> OUT_OF_RESOURCES; n == 0 -> SUCCESS without a launch.
- * No book is read or written. */
+ * Lists that name a page as a destination twice, or both as a source and as a
+ * destination, leave the bytes of that page undefined, as overlapping copies do.
+ * The pools may have been made on two handles of one GPU; `dst`'s is the one
+ * whose stream NULL means.  NULL list with n > 0, pools that differ ->
+ * INVALID_ARGUMENT; n pages of 2^32 pieces of 1 KiB or more ->
+ * OUT_OF_RESOURCES; n == 0 -> SUCCESS without a launch.  No book is read or
+ * written. */
 int mi355_blit_pages_copy(mi355_blit_pages_t* dst, const int32_t* dst_pages, mi355_blit_pages_t* src,
                           const int32_t* src_pages, const int32_t* valid_rows, size_t n, uint32_t route,
                           void* stream);

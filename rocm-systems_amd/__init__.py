@@ -1,5 +1,5 @@
-"""gfx950 blit engine: linear copy, dword fill and batched small copies on one
-MI355X, behind the interface of ROCr's core::Blit.
+"""gfx950 blit engine: linear copy, dword fill, batched small copies and the pages
+of a key/value cache on one MI355X, behind the interface of ROCr's core::Blit.
 
 The directory name contains a hyphen, so it is imported by path under the
 module name ``rocm_systems_amd`` (see ``__graft_entry__.load_package``).

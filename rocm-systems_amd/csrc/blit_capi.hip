@@ -1018,8 +1018,10 @@ int mi355_blit_pages_reset(mi355_blit_pages_t* p, void* stream) {
   std::lock_guard<std::mutex> g(p->h->lock);
   DeviceScope scope(p->h->device);
   if (scope.err != hipSuccess) return status_of(scope.err);
-  const PageResetArgs a{p->book, p->book_words};
-  hipLaunchKernelGGL(mi355_pages_reset, dim3(static_cast<uint32_t>((p->book_words + 255) / 256)), dim3(256), 0,
+  const uint64_t want = (p->book_words + 255) / 256;
+  const uint32_t grid = want < 65536 ? static_cast<uint32_t>(want) : 65536;
+  const PageResetArgs a{p->book, p->book_words, grid * 256ull};
+  hipLaunchKernelGGL(mi355_pages_reset, dim3(grid), dim3(256), 0,
                      stream ? static_cast<hipStream_t>(stream) : p->h->stream, a);
   BLIT_HIP(hipGetLastError());
   return MI355_BLIT_SUCCESS;

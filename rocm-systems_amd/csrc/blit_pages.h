@@ -20,8 +20,8 @@ namespace mi355 {
 // A wave moves a piece of a page at a time: 16 bytes for each lane, or four
 // times that where the first rows of the pages are moved only, so that fewer
 // waves find nothing to do (190 pages of 24 planes, half of their rows: 13.3 us
-// against 15.8; 600 pages of 1 MiB 134 against 153; whole pages, 800 of 1 MiB:
-// 285 us with 1 KiB, 330 with 4 KiB).
+// against 15.8; 600 pages of 1 MiB, half of their rows: 134 against 153; whole
+// pages, 800 of 1 MiB: 285 us with 1 KiB, 330 with 4 KiB).
 constexpr unsigned kPieceUnrolls[] = {1, 4};
 constexpr uint32_t piece_bytes(unsigned unroll) { return kWave * 16 * unroll; }
 
@@ -169,6 +169,7 @@ struct PageCompactFinishArgs {
 struct PageResetArgs {
   BookPtrs book;
   uint64_t words;  // of the whole buffer
+  uint64_t lanes;  // of the launch
 };
 
 // The free bits as the first launch of a reservation or a compaction takes
@@ -332,31 +333,33 @@ struct PageMovePlan {
 };
 
 // How n moves are launched; most_per_cu not 0: n is what a list has room for,
-// the device knows how many there are, and this many workgroups for each CU are the most.  pieces: of a page, for each size of piece.
+// the device knows how many there are, and this many workgroups for each CU are
+// the most.  pieces: of a page, for each size of piece.
 //
 // Cache policy, by the bytes that are likely moved (half of the pages where only
-// their first rows are).  Measured, pages of 32 planes of 32 KiB, loads and stores cached /
-// non-temporal loads with stores written through / with non-temporal stores:
-// 64 MiB 22.8 / 22.0 / 27.7 us, 128 MiB 42.9 / 41.9 / 51.0, 192 MiB 79.2 / 61.0 /
-// 74.2, 256 MiB 106.7 / 83.1 / 98.5, 384 MiB 156 / 153 / 143, 600 MiB 237 / 239 / 221.
+// their first rows are).  Measured, pages of 32 planes of 32 KiB, loads and
+// stores cached / non-temporal loads with stores written through / with
+// non-temporal stores: 64 MiB 22.8 / 22.0 / 27.7 us, 128 MiB 42.9 / 41.9 / 51.0,
+// 192 MiB 79.2 / 61.0 / 74.2, 256 MiB 106.7 / 83.1 / 98.5, 384 MiB 156 / 153 / 143,
+// 600 MiB 237 / 239 / 221.
 //
 // A wave for each piece: the dispatcher hands pieces out in order, which keeps
-// what is in flight close together (1 GiB, 32 KiB a page and plane: 369 us; a
-// grid of 8 workgroups for each CU whose waves stride 446, and 425 with the next piece's loads
-// in front of the stores).  A list of unknown length is as long as its room: a
-// wave too many costs 0.05 ns, so kMostListed workgroups for each CU (26 us of them
-// at most), and strides beyond (800 MiB 292 us; with 128 for each CU 325).
-// Over the host link at most link_grid workgroups, as for the linear copy; what
+// what is in flight close together (1 GiB, 32 KiB a page and plane: 369 us; with 32
+// workgroups for each CU whose waves stride 425, and 422 with the next piece's
+// loads in front of the stores).  A list of unknown length is as long as its
+// room: a wave too many costs 0.05 ns, so kMostListed workgroups for each CU (26
+// us of them at most), and strides beyond (800 MiB 292 us; with 128 for each CU
+// 325).  A reservation's list is as long as the call's and mostly empty:
+// kMostReserved for each CU (256 copies of 16 KiB in 32 planes 27.5 us; a wave
+// for each piece 25.5, and 6 us where nothing is copied).  Over the host link at
+// most link_grid workgroups, as for the linear copy (57 GB/s either way); what
 // goes to the host is written through at once.
-// A reservation's list is as long as the call's and mostly empty: kMostReserved
-// for each CU (256 copies of 16 KiB in 32 planes 27.5 us, 25.5 with a wave for each piece,
-// which costs 6 us where nothing is copied).
 constexpr uint32_t kMoveWaves = 4;
 constexpr uint32_t kMostListed = 512, kMostReserved = 16;
 constexpr uint64_t kMoveStreams = 128ull << 20, kMoveNtStores = 320ull << 20;
 
-inline PageMovePlan plan_page_moves(uint64_t n, uint32_t most_per_cu, bool cut, const uint32_t (&pieces)[2], uint64_t page_bytes,
-                                    uint32_t num_cus, uint32_t route, uint32_t link_grid) {
+inline PageMovePlan plan_page_moves(uint64_t n, uint32_t most_per_cu, bool cut, const uint32_t (&pieces)[2],
+                                    uint64_t page_bytes, uint32_t num_cus, uint32_t route, uint32_t link_grid) {
   PageMovePlan p;
   p.table = cut ? 1 : 0;
   const uint64_t bytes = cut ? n * page_bytes / 2 : n * page_bytes;
@@ -366,7 +369,8 @@ inline PageMovePlan plan_page_moves(uint64_t n, uint32_t most_per_cu, bool cut, 
                    : bytes >= kMoveStreams ? MI355_BLIT_STORE_AGENT_WT : MI355_BLIT_STORE_CACHED;
   const uint64_t want = (n * pieces[p.table] + kMoveWaves - 1) / kMoveWaves;
   const uint64_t most = route != MI355_BLIT_ROUTE_DEVICE ? link_grid
-                        : most_per_cu ? static_cast<uint64_t>(num_cus) * most_per_cu : kMaxGridWorkItems / (kMoveWaves * kWave);
+                        : most_per_cu ? static_cast<uint64_t>(num_cus) * most_per_cu
+                                      : kMaxGridWorkItems / (kMoveWaves * kWave);
   p.grid = static_cast<uint32_t>(want < most ? want : most);
   return p;
 }

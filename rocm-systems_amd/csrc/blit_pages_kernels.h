@@ -17,8 +17,10 @@ namespace mi355 {
 // ---------------------------------------------------------------------------
 // Moves.  One wave moves one piece of a page.  Work items go through the
 // planes one after the other, in each through the moves, and in each move through
-// the pieces of the page.  Bound by memory: 2 bytes of traffic for each byte of
-// the pages that are named, nothing else.
+// the pieces of the page: what is in flight then lies in one plane, some tens of
+// MiB, and not in all of them (512 pages of 64 planes of 32 KiB, 1 GiB each way: 369 us,
+// 5.8 TB/s, against 403 us in the order move, plane, piece; a linear copy of as many bytes 313).
+// Bound by memory: the counters show as many bytes read and written as the pages have.
 // ---------------------------------------------------------------------------
 
 // A page of several runs of which only the first rows are moved, `limit` bytes
@@ -99,8 +101,10 @@ MI355_DEVICE void page_move_body(const PageMoveArgs& a, uint64_t first_wave) {
       if (valid < a.rows) {
         const unsigned limit = valid * d.row_bytes;
         if (d.run_bytes) {
-          if ((limit | d.run_bytes) % 16 == 0) move_cut_runs<U, NTL, ST>(dp - offset, sp - offset, d, offset, limit, lane);
-          else move_odd_runs<NTL, ST>(dp, sp, d, offset, bytes, limit, lane);
+          if ((limit | d.run_bytes) % 16 == 0)
+            move_cut_runs<U, NTL, ST>(dp - offset, sp - offset, d, offset, limit, lane);
+          else
+            move_odd_runs<NTL, ST>(dp, sp, d, offset, bytes, limit, lane);
           continue;
         }
         if (limit <= offset) continue;
@@ -229,7 +233,10 @@ MI355_DEVICE void hand_out(const BookPtrs& b, uint32_t page, uint32_t nth, uint3
 // the second launch does, over the whole device, next to the copies.
 //
 // Bound by latency: a chain of dependent loads (entry, length, last page,
-// its count, free bits) and a dozen barriers.
+// its count, free bits) and a dozen barriers.  48 sequences that get a token each
+// 5.9 us and 2 for the second launch; 300 prompts, 19,000 pages 7.2 and 4.6 (one
+// workgroup that hands out all of them itself 244); 256 forks of 32 prompts of which 224
+// copy their last page 9.1, and 18.3 for 115 MB of copies (6.3 TB/s).
 MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
   MI355_LDS uint32_t scan_a[16], scan_b[16];
   MI355_LDS uint32_t keys[kSlots], first[kSlots], asked[kSlots];
@@ -375,7 +382,8 @@ MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
         for (unsigned k = 0; k < 4; ++k) {
           const uint32_t here = popcount32(bits.word[k]);
           if (left == 0 || here == 0) continue;
-          st_u32(b.bits + 4 * v + k, here <= left ? 0 : bits.word[k] >> nth_bit(bits.word[k], left) << nth_bit(bits.word[k], left));
+          const uint32_t kept_from = here <= left ? 0 : nth_bit(bits.word[k], left);
+          st_u32(b.bits + 4 * v + k, here <= left ? 0 : bits.word[k] >> kept_from << kept_from);
           left -= here <= left ? here : left;
         }
       }
@@ -483,18 +491,20 @@ MI355_DEVICE FourPages load_four(const int32_t* table, uint32_t j, uint32_t end)
 }
 
 // A sequence that holds its parent's pages.  A workgroup for each entry.  Each
-// reads the whole list (it is short and in L2), and so decides
-// without what another may already have written: a child that an earlier entry
-// names too is left alone, and so is one whose parent is named as a child.
+// reads the whole list (it is short and in L2), and so decides without what
+// another may already have written: a child that an earlier entry names too is
+// left alone, and so is one whose parent is named as a child.
 //
-// The atomic additions are what it takes time for (20 of them in a nanosecond, whatever
-// their addresses), so the first entry that names a parent adds to its pages'
-// counts for all that do; an entry that is refused for its child's sake, which the
-// others cannot see, takes its own share off again.  1000 children of 90 parents,
-// 560 pages each: 27.5 us with an addition for each child and page.
+// The atomic additions are what takes time (the device does 20 of them in a
+// nanosecond, whatever their addresses), so the first entry that names a parent
+// adds to its pages' counts for all that do; an entry that is refused for its
+// child's sake, which the others cannot see, takes its own share off again.
+// 1000 children of 90 parents, 560 pages each: 8.0 us, and 27.5 with an addition
+// for each child and page; 64 children of 16 parents 3.7.
 //
 // Where tables are long (a.made not null) an entry has a workgroup for each
-// a.chunk pages, nobody writes a length, and another launch does.
+// a.chunk pages, nobody writes a length, and another launch does (one child of
+// 98,000 pages: 11 us together).
 MI355_DEVICE void page_fork_body(const PageForkArgs& a) {
   MI355_LDS uint32_t parent_named, again, first, holders;
   const BookPtrs& b = a.book;
@@ -563,7 +573,7 @@ MI355_DEVICE void page_fork_lengths_body(const PageForkArgs& a) {
 // The end of a sequence, or of its tokens from `keep` on.  A workgroup for each
 // entry; lane 0 takes the sequence's tokens with an atomic minimum, so that of
 // two entries for one sequence each gives back what the other has not.  Bound by
-// latency: entry, minimum, table, count, free bits.
+// latency: entry, minimum, table, count, free bits (5 sequences 4.4 us).
 MI355_DEVICE void page_free_body(const PageFreeArgs& a) {
   MI355_LDS uint32_t before;
   const BookPtrs& b = a.book;
@@ -601,11 +611,13 @@ MI355_DEVICE void page_free_body(const PageFreeArgs& a) {
 }
 
 // The same for many pages, in two launches.  The device does some 20 atomics in
-// a nanosecond, so there is one for each page, whose result nobody waits for, and the
-// second launch makes the free bits from the counts and shortens the sequences
-// (306,000 pages of 850 sequences: 28 us with the free bits by atomics, 16 so).  A
-// workgroup for each entry and a.chunk pages of its table; the first entry that
-// names a sequence acts for all that do, with the smallest keep of theirs.
+// a nanosecond, so there is one for each page, whose result nobody waits for, and
+// the second launch makes the free bits from the counts and shortens the
+// sequences (306,000 pages of 850 sequences: 28 us with the free bits by atomics,
+// 17 so; the tails of 850 sequences that share their pages, 150,000 pages in all,
+// 9.6 and 2.3 us).  A workgroup for each entry and a.chunk pages of its table; the
+// first entry that names a sequence acts for all that do, with the smallest keep
+// of theirs.
 MI355_DEVICE void page_free_counts_body(const PageFreeArgs& a) {
   MI355_LDS uint32_t again, least;
   const BookPtrs& b = a.book;
@@ -665,7 +677,9 @@ MI355_DEVICE void page_free_finish_body(const PageFreeArgs& a) {
 // moves the bytes, next to workgroups that rewrite the tables and the free bits.
 // Beyond, the first launch leaves the free pages in front of each two words of
 // the free bits and how many pages move, and one between the two, over the
-// whole device, finds for each hole the page that comes to it.
+// whole device, finds for each hole the page that comes to it.  Bound by memory
+// where much moves (3,500 pages of 1 MiB of which 830 move: 4.6, 4.7 and 274 us,
+// 6.2 TB/s), by the launches otherwise (24 of 3,000 pages: 4.8 and 5.0 us).
 
 // Move k, of page `from` to page `to`: the list, the counts, and what the caller wants to know.
 MI355_DEVICE void list_move(const PageCompactArgs& a, uint32_t k, uint32_t from, uint32_t to) {
@@ -716,7 +730,8 @@ MI355_DEVICE void page_compact_plan_body(const PageCompactArgs& a) {
     st_obj(b.head, static_cast<int32_t>(n));
   }
   if (a.max_moves <= kListedAtOnce && t < n)
-    list_move(a, t, select_page<false>(b, groups, a.lane_vecs, live - 1 - t), select_page<true>(b, groups, a.lane_vecs, t));
+    list_move(a, t, select_page<false>(b, groups, a.lane_vecs, live - 1 - t),
+              select_page<true>(b, groups, a.lane_vecs, t));
 }
 
 // The counts of the pages that move and where they go.
@@ -737,7 +752,8 @@ MI355_DEVICE void page_compact_list_body(const PageCompactArgs& a) {
     uint32_t lo = 0, hi = a.n_pairs;  // [lo, hi) holds it
     while (hi - lo > 1) {
       const uint32_t mid = (lo + hi) / 2;
-      if (64 * mid - ld_u32<false>(a.pairs + mid) <= rank) lo = mid; else hi = mid;
+      if (64 * mid - ld_u32<false>(a.pairs + mid) <= rank) lo = mid;
+      else hi = mid;
     }
     uint32_t r = rank - (64 * lo - ld_u32<false>(a.pairs + lo));
     const uint32_t w0 = ~ld_u32<false>(b.bits + 2 * lo);
@@ -795,7 +811,7 @@ MI355_DEVICE void page_compact_finish_body(const PageCompactFinishArgs& f) {
   else if (wg < a.pair_wgs + a.book.max_seqs)
     page_compact_tables_body(a, n, wg - a.pair_wgs);
   else
-    page_move_body<1, NTL, ST>(f.moves, global_wave(kMoveWaves) - (a.pair_wgs + a.book.max_seqs) * static_cast<uint64_t>(kMoveWaves));
+    page_move_body<1, NTL, ST>(f.moves, global_wave(kMoveWaves) - static_cast<uint64_t>(kMoveWaves) * (a.pair_wgs + a.book.max_seqs));
 }
 
 // An empty book: no tokens, no holders, every page free, no table entry.
@@ -803,16 +819,16 @@ MI355_DEVICE void page_reset_body(const PageResetArgs& a) {
   const BookPtrs& b = a.book;
   const int64_t bits_at = reinterpret_cast<int32_t*>(b.bits) - b.head;
   const int64_t tables_at = b.tables - b.head;
-  const uint64_t i = static_cast<uint64_t>(workgroup_index()) * 256 + thread_in_workgroup();
-  if (i >= a.words) return;
-  uint32_t v = 0;
-  if (static_cast<int64_t>(i) >= tables_at) {
-    v = ~0u;
-  } else if (static_cast<int64_t>(i) >= bits_at) {
-    const uint64_t page = 32 * (i - bits_at);
-    if (page < b.num_pages) v = b.num_pages - page >= 32 ? ~0u : (1u << (b.num_pages - page)) - 1;
+  for (uint64_t i = static_cast<uint64_t>(workgroup_index()) * 256 + thread_in_workgroup(); i < a.words; i += a.lanes) {
+    uint32_t v = 0;
+    if (static_cast<int64_t>(i) >= tables_at) {
+      v = ~0u;
+    } else if (static_cast<int64_t>(i) >= bits_at) {
+      const uint64_t page = 32 * (i - bits_at);
+      if (page < b.num_pages) v = b.num_pages - page >= 32 ? ~0u : (1u << (b.num_pages - page)) - 1;
+    }
+    st_obj(b.head + i, static_cast<int32_t>(v));
   }
-  st_obj(b.head + i, static_cast<int32_t>(v));
 }
 
 }  // namespace mi355

@@ -167,7 +167,8 @@ struct Cache {
     moves = pages_move_list(work, w);
     reserving = pages_reserve_work(work, w);
     start();
-    run(mi355_pages_reset, PageResetArgs{ptrs, at.words}, static_cast<uint32_t>((at.words + 255) / 256), 256);
+    const uint32_t grid = 1 + static_cast<uint32_t>(below((at.words + 255) / 256));
+    run(mi355_pages_reset, PageResetArgs{ptrs, at.words, grid * 256ull}, grid, 256);
     lengths.assign(c.seqs, 0);
     refs.assign(c.pages, 0);
     tables.assign(static_cast<size_t>(c.seqs) * c.width, -1);
