@@ -142,7 +142,7 @@ MI355_DEVICE uint32_t count_bits(const BitTile& t) {
   return popcount32(t.word[0]) + popcount32(t.word[1]) + popcount32(t.word[2]) + popcount32(t.word[3]);
 }
 
-// A table in LDS that finds equal keys among the 1024 entries of a round: open
+// A table in LDS that finds equal keys among the 1024 entries of a turn: open
 // addressing over twice as many slots, so that a free one is always found.
 constexpr uint32_t kSlots = 2048;
 constexpr uint32_t kNoKey = ~0u;
@@ -220,12 +220,49 @@ MI355_DEVICE void hand_out(const BookPtrs& b, uint32_t page, uint32_t nth, uint3
   st_obj(b.refs + page, 1);
 }
 
+// An entry of a reservation with what the book says of its sequence.
+struct ReserveEntry {
+  uint32_t seq, tokens, old_pages, new_pages;
+  int32_t more;
+  bool valid;      // but for an earlier entry of the sequence
+  uint32_t fill;   // rows in use on the last page
+  uint32_t tail;   // the last page, where it has room and rows are to be added
+  uint32_t holders;  // of the tail; 0 where there is none
+};
+
+// `changed`: earlier turns of the call may have changed the counts.
+MI355_DEVICE ReserveEntry load_reserve_entry(const PageReserveArgs& a, uint32_t i, bool changed) {
+  const BookPtrs& b = a.book;
+  ReserveEntry e{~0u, 0, 0, 0, 0, false, 0, 0, 0};
+  if (i >= a.n) return e;
+  e.seq = static_cast<uint32_t>(ld_obj(a.seqs + i));
+  e.more = ld_obj(a.add + i);
+  if (e.seq >= b.max_seqs) return e;
+  e.tokens = ld_obj(b.lengths + e.seq);
+  if (e.more < 0 || static_cast<int32_t>(e.tokens) < 0) return e;
+  // both below 2^31, so the sum is below 2^32
+  e.old_pages = pages_held(e.tokens, b);
+  e.new_pages = pages_held(e.tokens + e.more, b);
+  if (e.new_pages > b.width) return e;
+  e.valid = true;
+  e.fill = e.tokens - div_magic(e.tokens, b.magic_rows) * b.rows;
+  if (e.more == 0 || e.fill == 0) return e;
+  e.tail = ld_obj(b.tables + static_cast<uint64_t>(e.seq) * b.width + e.old_pages - 1);
+  if (e.tail >= b.num_pages) {
+    e.valid = false;  // not a page
+    return e;
+  }
+  e.holders = changed ? ld_agent_u32(reinterpret_cast<const uint32_t*>(b.refs + e.tail))
+                      : static_cast<uint32_t>(ld_obj(b.refs + e.tail));
+  return e;
+}
+
 // Room for new tokens, in two launches, so that the result is that of taking
 // the entries one by one.
 //
 // The first, one workgroup of 1024 lanes, takes the entries 1024 at a time:
 // which of them name a sequence first (a table in LDS, and a bit for each
-// sequence that an earlier round named), which of them have to copy a last page
+// sequence that an earlier turn named), which of them have to copy a last page
 // that others hold as well, how many pages each needs and how many the entries
 // before it get, out of how many free ones.  The k-th lowest free page goes to the
 // entry whose share of the running sum k falls into.  Where the pages are no
@@ -234,9 +271,9 @@ MI355_DEVICE void hand_out(const BookPtrs& b, uint32_t page, uint32_t nth, uint3
 //
 // Bound by latency: a chain of dependent loads (entry, length, last page,
 // its count, free bits) and a dozen barriers.  48 sequences that get a token each
-// 5.9 us and 2 for the second launch; 300 prompts, 19,000 pages 7.2 and 4.6 (one
+// 5.6 us and 2 for the second launch; 300 prompts, 19,000 pages 7.1 and 4.9 (one
 // workgroup that hands out all of them itself 244); 256 forks of 32 prompts of which 224
-// copy their last page 9.1, and 18.3 for 115 MB of copies (6.3 TB/s).
+// copy their last page 9.0, and 18.3 for 115 MB of copies (6.3 TB/s).
 MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
   MI355_LDS uint32_t scan_a[16], scan_b[16];
   MI355_LDS uint32_t keys[kSlots], first[kSlots], asked[kSlots];
@@ -246,19 +283,23 @@ MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
   const BookPtrs& b = a.book;
   const uint32_t t = thread_in_workgroup();
 
+  // The first entries' loads are under way while the free bits are summed up.
+  ReserveEntry mine = load_reserve_entry(a, t, false);
   // the free bits, a stretch for each lane
   const BitTile kept = load_bits_vec(b, t * a.lane_vecs);
-  uint32_t mine = count_bits(kept);
-  for (uint32_t k = 1; k < a.lane_vecs; ++k) mine += count_bits(load_bits_vec(b, t * a.lane_vecs + k));
+  uint32_t bits_here = count_bits(kept);
+  for (uint32_t k = 1; k < a.lane_vecs; ++k) bits_here += count_bits(load_bits_vec(b, t * a.lane_vecs + k));
+  for (uint32_t k = t; k < kSlots; k += 1024) keys[k] = kNoKey, first[k] = ~0u;
   if (a.n > 1024)
     for (uint32_t k = t; k < kMaxSeqs / 32; k += 1024) seen[k] = 0;
-  if (t == 0) n_moves = 0, handed = 0;
+  if (t == 0) n_moves = 0, handed = 0, any_shared = 0, any_refused = 0;
   uint32_t free_pages;
-  const uint32_t in_front = block_scan_1024(mine, scan_b, &free_pages);
+  const uint32_t in_front = block_scan_1024(bits_here, scan_b, &free_pages);
   groups[t] = in_front;
 
-  bool stopped = false;  // the same in all lanes
-  uint32_t carry = 0;    // pages that earlier rounds get
+  bool stopped = false;  // the same in all lanes, as are the next two
+  uint32_t carry = 0;    // pages that earlier turns get
+  uint32_t left_over = 0;  // pages that the second launch hands out
   for (uint32_t base = 0; base < a.n; base += 1024) {
     const uint32_t i = base + t;
     if (stopped) {
@@ -268,50 +309,37 @@ MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
       }
       continue;
     }
-    const uint32_t s = i < a.n ? static_cast<uint32_t>(ld_obj(a.seqs + i)) : ~0u;
-    const int32_t more = i < a.n ? ld_obj(a.add + i) : 0;
-    for (uint32_t k = t; k < kSlots; k += 1024) keys[k] = kNoKey, first[k] = ~0u;
-    if (t == 0) any_shared = 0, any_refused = 0;
-    workgroup_barrier();
-
+    if (base) {
+      mine = load_reserve_entry(a, i, true);
+      for (uint32_t k = t; k < kSlots; k += 1024) keys[k] = kNoKey, first[k] = ~0u;
+      if (t == 0) any_shared = 0, any_refused = 0;
+      workgroup_barrier();
+    }
+    const uint32_t s = mine.seq, tokens = mine.tokens, fill = mine.fill, tail = mine.tail, holders = mine.holders;
+    const int32_t more = mine.more;
     const bool named = s < b.max_seqs;
-    uint32_t slot = 0, tokens = 0;
+    uint32_t slot = 0;
     bool again = false;
     if (named) {
-      tokens = ld_obj(b.lengths + s);
       again = base && (seen[s / 32] >> (s % 32) & 1);
       slot = hash_slot(keys, s);
       lds_min(first + slot, t);
     }
+    // (perhaps by an entry that is refused)
+    if (static_cast<int32_t>(holders) > 1) any_shared = 1;
     workgroup_barrier();
     if (named) {
       again = again || first[slot] != t;
       if (a.n > 1024) lds_or(seen + s / 32, 1u << (s % 32));
     }
-    // both below 2^31, so the sum is below 2^32
-    const uint32_t old_pages = pages_held(tokens, b);
-    const uint32_t new_pages = more >= 0 ? pages_held(tokens + more, b) : 0;
-    bool ok = named && !again && more >= 0 && static_cast<int32_t>(tokens) >= 0 && new_pages <= b.width;
-    const uint32_t fill = tokens - div_magic(tokens, b.magic_rows) * b.rows;
-    bool shared = false;
-    uint32_t tail = 0, holders = 0;
-    if (ok && more > 0 && fill != 0) {
-      tail = ld_obj(b.tables + static_cast<uint64_t>(s) * b.width + old_pages - 1);
-      if (tail < b.num_pages) {
-        // an earlier round may have changed it
-        holders = base ? ld_agent_u32(reinterpret_cast<const uint32_t*>(b.refs + tail))
-                       : static_cast<uint32_t>(ld_obj(b.refs + tail));
-        shared = static_cast<int32_t>(holders) > 1;
-      } else {
-        ok = false;  // not a page
-      }
-    }
-    if (shared) any_shared = 1;
-    workgroup_barrier();
+    const uint32_t old_pages = mine.old_pages, new_pages = mine.new_pages;
+    const bool ok = mine.valid && !again;
+    const bool shared = ok && static_cast<int32_t>(holders) > 1;
     bool copies = shared;
     uint32_t leavers = 0;  // not 0 in one of the askers of a page: how many of them copy it
     if (any_shared) {
       // With as many askers as holders, the last of them finds the page its own.
+      workgroup_barrier();  // the table of sequences has been read
       for (uint32_t k = t; k < kSlots; k += 1024) keys[k] = kNoKey, first[k] = 0, asked[k] = 0;
       workgroup_barrier();
       if (shared) {
@@ -387,20 +415,19 @@ MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
           left -= here <= left ? here : left;
         }
       }
-      if (t == 0) handed = 0;
     } else {
       if (i < a.n) {
         st_u32(a.work.start + i, start[t]);
         st_u32(a.work.who + i, who[t]);
         st_u32(a.work.slot + i, slot_of[t]);
       }
-      carry = wanted;
-      // the next round reads counts that this one wrote
+      carry = left_over = wanted;
+      // the next turn reads counts that this one wrote
       if (base + 1024 < a.n) wait_for_memory();
+      workgroup_barrier();
     }
-    workgroup_barrier();
   }
-  if (handed) {
+  if (left_over) {
     uint32_t front = in_front;
     for (uint32_t k = 0; k < a.lane_vecs; ++k) {
       const uint32_t v = t * a.lane_vecs + k;
@@ -414,7 +441,7 @@ MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
   }
   if (t == 0) {
     st_obj(a.moves.count, PageMoveCount{n_moves, 0, magic_divisor(n_moves)});
-    st_u32(a.work.wanted, handed);
+    st_u32(a.work.wanted, left_over);
   }
 }
 
@@ -473,7 +500,7 @@ MI355_DEVICE void page_finish_body(const PageFinishArgs& a) {
     page_move_body<4, NTL, ST>(a.moves, global_wave(kMoveWaves) - a.assign_wgs * kMoveWaves);
 }
 
-// Table entries j .. j + 3 of a sequence, those below `end`.
+// Entries j .. j + 3 of a table or a list, those below `end` (~0 for the others).
 struct FourPages {
   uint32_t page[4];
 };
@@ -499,8 +526,8 @@ MI355_DEVICE FourPages load_four(const int32_t* table, uint32_t j, uint32_t end)
 // nanosecond, whatever their addresses), so the first entry that names a parent
 // adds to its pages' counts for all that do; an entry that is refused for its
 // child's sake, which the others cannot see, takes its own share off again.
-// 1000 children of 90 parents, 560 pages each: 8.0 us, and 27.5 with an addition
-// for each child and page; 64 children of 16 parents 3.7.
+// 1000 children of 90 parents, 560 pages each: 7.8 us, and 27.5 with an addition
+// for each child and page; 64 children of 16 parents 4.1.
 //
 // Where tables are long (a.made not null) an entry has a workgroup for each
 // a.chunk pages, nobody writes a length, and another launch does (one child of
@@ -528,13 +555,15 @@ MI355_DEVICE void page_fork_body(const PageForkArgs& a) {
   if (chunk != 0 && chunk * a.chunk >= held) return;
   workgroup_barrier();
   uint32_t mine = 0;
-  for (uint32_t k = t; k < a.n; k += a.wg_size) {
-    const uint32_t p = static_cast<uint32_t>(ld_obj(a.parents + k));
-    const uint32_t c = static_cast<uint32_t>(ld_obj(a.children + k));
-    if (c == parent) parent_named = 1;
-    if (c == child && k < i) again = 1;
-    if (p == parent && c < b.max_seqs) {
-      if (mine++ == 0) lds_min(&first, k);
+  for (uint32_t k = 4 * t; k < a.n; k += 4 * a.wg_size) {
+    const FourPages p = load_four(a.parents, k, a.n), c = load_four(a.children, k, a.n);
+#pragma unroll
+    for (unsigned u = 0; u < 4; ++u) {
+      if (c.page[u] == parent) parent_named = 1;
+      if (c.page[u] == child && k + u < i) again = 1;
+      if (p.page[u] == parent && c.page[u] < b.max_seqs) {
+        if (mine++ == 0) lds_min(&first, k + u);
+      }
     }
   }
   if (mine) lds_add(&holders, mine);
@@ -615,7 +644,7 @@ MI355_DEVICE void page_free_body(const PageFreeArgs& a) {
 // the second launch makes the free bits from the counts and shortens the
 // sequences (306,000 pages of 850 sequences: 28 us with the free bits by atomics,
 // 17 so; the tails of 850 sequences that share their pages, 150,000 pages in all,
-// 9.6 and 2.3 us).  A workgroup for each entry and a.chunk pages of its table; the
+// 9.5 and 2.3 us).  A workgroup for each entry and a.chunk pages of its table; the
 // first entry that names a sequence acts for all that do, with the smallest keep
 // of theirs.
 MI355_DEVICE void page_free_counts_body(const PageFreeArgs& a) {
@@ -632,23 +661,31 @@ MI355_DEVICE void page_free_counts_body(const PageFreeArgs& a) {
   if (chunk * a.chunk >= end) return;
   if (t == 0) again = 0, least = ~0u;
   workgroup_barrier();
-  for (uint32_t k = t; k < a.n; k += a.wg_size) {
-    if (static_cast<uint32_t>(ld_obj(a.seqs + k)) != s) continue;
-    // a negative number is a large unsigned one
-    lds_min(&least, a.keep ? static_cast<uint32_t>(ld_obj(a.keep + k)) : 0);
-    if (k < i) again = 1;
+  if (end > (chunk + 1) * a.chunk) end = (chunk + 1) * a.chunk;
+  const int32_t* table = b.tables + static_cast<uint64_t>(s) * b.width;
+  // the first entries of the stretch are under way while the list is read
+  uint32_t j = chunk * a.chunk + 4 * t;
+  FourPages f;
+  if (j < end) f = load_four(table, j, end);
+  for (uint32_t k = 4 * t; k < a.n; k += 4 * a.wg_size) {
+    const FourPages named = load_four(a.seqs, k, a.n);
+#pragma unroll
+    for (unsigned u = 0; u < 4; ++u) {
+      if (named.page[u] != s) continue;
+      // a negative number is a large unsigned one
+      lds_min(&least, a.keep ? static_cast<uint32_t>(ld_obj(a.keep + k + u)) : 0);
+      if (k + u < i) again = 1;
+    }
   }
   workgroup_barrier();
   if (again || least >= static_cast<uint32_t>(tokens)) return;
-  uint32_t j = pages_held(least, b);
-  if (j < chunk * a.chunk) j = chunk * a.chunk;
-  if (end > (chunk + 1) * a.chunk) end = (chunk + 1) * a.chunk;
-  const int32_t* table = b.tables + static_cast<uint64_t>(s) * b.width;
-  for (j += 4 * t; j < end; j += 4 * a.wg_size) {
-    const FourPages f = load_four(table, j, end);
+  const uint32_t from = pages_held(least, b);
+  while (j < end) {
 #pragma unroll
     for (unsigned k = 0; k < 4; ++k)
-      if (f.page[k] < b.num_pages) add_agent_i32(b.refs + f.page[k], -1);
+      if (j + k >= from && f.page[k] < b.num_pages) add_agent_i32(b.refs + f.page[k], -1);
+    j += 4 * a.wg_size;
+    if (j < end) f = load_four(table, j, end);
   }
 }
 
@@ -678,7 +715,7 @@ MI355_DEVICE void page_free_finish_body(const PageFreeArgs& a) {
 // Beyond, the first launch leaves the free pages in front of each two words of
 // the free bits and how many pages move, and one between the two, over the
 // whole device, finds for each hole the page that comes to it.  Bound by memory
-// where much moves (3,500 pages of 1 MiB of which 830 move: 4.6, 4.7 and 274 us,
+// where much moves (3,500 pages of 1 MiB of which 815 move: 4.6, 4.7 and 274 us,
 // 6.2 TB/s), by the launches otherwise (24 of 3,000 pages: 4.8 and 5.0 us).
 
 // Move k, of page `from` to page `to`: the list, the counts, and what the caller wants to know.

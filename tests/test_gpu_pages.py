@@ -398,9 +398,9 @@ def test_a_list_of_the_longest_kind(torch_cuda, capi, engine, rand):
         c.close()
 
 
-def test_holders_of_a_page_in_different_rounds_of_a_list(torch_cuda, capi, engine, rand):
-    """A list is taken 1024 entries at a time: what an earlier round has left of a page's
-    holders is what a later one finds."""
+def test_holders_of_a_page_far_apart_in_a_list(torch_cuda, capi, engine, rand):
+    """A list is taken 1024 entries at a time: what the first have left of a page's holders is
+    what later ones find."""
     n = 2600
     c = Cache(torch_cuda, capi, engine, rand, 12000, 16, 3 * n, 2, [(4, 1, 0, 0)])
     try:
@@ -445,6 +445,74 @@ def test_other_streams(torch_cuda, capi, engine, rand):
         c.compact(10)
     finally:
         c.close()
+
+
+def test_two_caches_at_once(torch_cuda, capi, engine, rand):
+    """Two threads, each with a cache and a stream of its own, calling the same handle."""
+    import threading
+    torch = torch_cuda
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    caches = [Cache(torch, capi, engine, rand, 300, 16, 24, 12, [(64, 1, 0, 0), (30, 3, 5, 1)], seed=k,
+                    stream=streams[k].cuda_stream) for k in range(2)]
+    failed = []
+
+    def live(k):
+        try:
+            rng = np.random.default_rng(40 + k)
+            for _ in range(25):
+                ids = [int(x) for x in rng.permutation(24)[:8]]
+                caches[k].reserve(ids, [int(x) for x in rng.integers(0, 40, 8)])
+                caches[k].fork(ids[:4], ids[4:])
+                caches[k].free(ids[2:5], [int(x) for x in rng.integers(0, 60, 3)])
+                caches[k].compact(int(rng.integers(1, 60)))
+        except BaseException as e:  # an assertion of another thread
+            failed.append((k, repr(e)))
+    try:
+        threads = [threading.Thread(target=live, args=(k,)) for k in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not failed, failed
+    finally:
+        for c in caches:
+            c.close()
+
+
+def test_graphs_of_two_caches_replayed_together(torch_cuda, capi, engine, rand):
+    """Each cache has work memory of its own: their graphs may run side by side."""
+    torch = torch_cuda
+    caches = [Cache(torch, capi, engine, rand, 5000, 4, 64, 60, [(64, 1, 0, 0)], seed=k) for k in range(2)]
+    try:
+        n = 40
+        seqs, more, keep = (caches[0].list(v) for v in (range(n), [70 + i for i in range(n)], [33 + i for i in range(n)]))
+        graphs = []
+        for c in caches:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+                s = torch.cuda.current_stream().cuda_stream
+                ok(capi, c.pages.reserve(seqs.data_ptr(), more.data_ptr(), n, None, s))
+                ok(capi, c.pages.free(seqs.data_ptr(), n, keep.data_ptr(), s))
+                ok(capi, c.pages.compact(400, None, s))
+            graphs.append(graph)
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        for replay in range(4):
+            for g, st in zip(graphs, streams):
+                with torch.cuda.stream(st):
+                    g.replay()
+            for c in caches:
+                m = c.model
+                c.move(m.reserve(list(range(n)), [70 + i for i in range(n)])[1])
+                m.free(list(range(n)), [33 + i for i in range(n)])
+                c.move([(f, t, c.rows) for f, t in m.compact(400)])
+            for c in caches:
+                c.check("replay %d" % replay)
+            for k, c in enumerate(caches):  # eager calls between the replays
+                c.free([5 + k, 11], [0, 3 * replay])
+        del graphs
+    finally:
+        for c in caches:
+            c.close()
 
 
 def test_calls_recorded_into_a_graph(torch_cuda, capi, engine, rand):
