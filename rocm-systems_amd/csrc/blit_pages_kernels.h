@@ -526,8 +526,8 @@ MI355_DEVICE FourPages load_four(const int32_t* table, uint32_t j, uint32_t end)
 // nanosecond, whatever their addresses), so the first entry that names a parent
 // adds to its pages' counts for all that do; an entry that is refused for its
 // child's sake, which the others cannot see, takes its own share off again.
-// 1000 children of 90 parents, 560 pages each: 7.8 us, and 27.5 with an addition
-// for each child and page; 64 children of 16 parents 4.1.
+// 1000 children of 90 parents, 560 pages each: 7.6 us, and 27.5 with an addition
+// for each child and page; 64 children of 16 parents 3.8.
 //
 // Where tables are long (a.made not null) an entry has a workgroup for each
 // a.chunk pages, nobody writes a length, and another launch does (one child of
@@ -546,6 +546,14 @@ MI355_DEVICE void page_fork_body(const PageForkArgs& a) {
     }
     return;
   }
+  // what is needed behind the barriers is under way in front of them: the
+  // lists, and the parent's table as if it were full
+  uint32_t k = 4 * t;
+  FourPages ps, cs, f;
+  if (k < a.n) ps = load_four(a.parents, k, a.n), cs = load_four(a.children, k, a.n);
+  const int32_t* from = b.tables + static_cast<uint64_t>(parent) * b.width;
+  uint32_t j = chunk * a.chunk + 4 * t;
+  if (j < b.width) f = load_four(from, j, b.width);
   if (t == 0) parent_named = 0, again = 0, first = ~0u, holders = 0;
   const uint32_t tokens = ld_obj(b.lengths + parent);
   // only the first entry that names the child writes it, after the barriers
@@ -555,33 +563,35 @@ MI355_DEVICE void page_fork_body(const PageForkArgs& a) {
   if (chunk != 0 && chunk * a.chunk >= held) return;
   workgroup_barrier();
   uint32_t mine = 0;
-  for (uint32_t k = 4 * t; k < a.n; k += 4 * a.wg_size) {
-    const FourPages p = load_four(a.parents, k, a.n), c = load_four(a.children, k, a.n);
+  while (k < a.n) {
 #pragma unroll
     for (unsigned u = 0; u < 4; ++u) {
-      if (c.page[u] == parent) parent_named = 1;
-      if (c.page[u] == child && k + u < i) again = 1;
-      if (p.page[u] == parent && c.page[u] < b.max_seqs) {
+      if (cs.page[u] == parent) parent_named = 1;
+      if (cs.page[u] == child && k + u < i) again = 1;
+      if (ps.page[u] == parent && cs.page[u] < b.max_seqs) {
         if (mine++ == 0) lds_min(&first, k + u);
       }
     }
+    k += 4 * a.wg_size;
+    if (k < a.n) ps = load_four(a.parents, k, a.n), cs = load_four(a.children, k, a.n);
   }
   if (mine) lds_add(&holders, mine);
   workgroup_barrier();
   const bool made = !parent_named && !again && !in_use;
   if (!parent_named) {
     const int32_t more = (first == i ? static_cast<int32_t>(holders) : 0) - (made ? 0 : 1);
-    const int32_t* from = b.tables + static_cast<uint64_t>(parent) * b.width;
     int32_t* to = b.tables + static_cast<uint64_t>(child) * b.width;
     uint32_t end = held;
     if (a.made && end > (chunk + 1) * a.chunk) end = (chunk + 1) * a.chunk;
-    for (uint32_t j = chunk * a.chunk + 4 * t; j < end; j += 4 * a.wg_size) {
-      const FourPages f = load_four(from, j, end);
+    while (j < end) {
 #pragma unroll
-      for (unsigned k = 0; k < 4; ++k) {
-        if (made && j + k < end) st_obj(to + j + k, static_cast<int32_t>(f.page[k]));
-        if (more && f.page[k] < b.num_pages) add_agent_i32(b.refs + f.page[k], more);
+      for (unsigned u = 0; u < 4; ++u) {
+        if (j + u >= end) continue;
+        if (made) st_obj(to + j + u, static_cast<int32_t>(f.page[u]));
+        if (more && f.page[u] < b.num_pages) add_agent_i32(b.refs + f.page[u], more);
       }
+      j += 4 * a.wg_size;
+      if (j < end) f = load_four(from, j, end);
     }
   }
   if (t != 0 || chunk != 0) return;
@@ -602,7 +612,7 @@ MI355_DEVICE void page_fork_lengths_body(const PageForkArgs& a) {
 // The end of a sequence, or of its tokens from `keep` on.  A workgroup for each
 // entry; lane 0 takes the sequence's tokens with an atomic minimum, so that of
 // two entries for one sequence each gives back what the other has not.  Bound by
-// latency: entry, minimum, table, count, free bits (5 sequences 4.4 us).
+// latency: entry, minimum, table, count, free bits (5 sequences 4.2 us).
 MI355_DEVICE void page_free_body(const PageFreeArgs& a) {
   MI355_LDS uint32_t before;
   const BookPtrs& b = a.book;
@@ -611,19 +621,22 @@ MI355_DEVICE void page_free_body(const PageFreeArgs& a) {
   const uint32_t s = static_cast<uint32_t>(ld_obj(a.seqs + i));
   const int32_t keep = a.keep ? ld_obj(a.keep + i) : 0;
   if (s >= b.max_seqs || keep < 0) return;
+  // the table as if it were full, while the minimum is under way
+  const int32_t* table = b.tables + static_cast<uint64_t>(s) * b.width;
+  uint32_t j = pages_held(keep, b) + 4 * t;
+  FourPages f;
+  if (j < b.width) f = load_four(table, j, b.width);
   if (t == 0) before = static_cast<uint32_t>(min_agent_i32(b.lengths + s, keep));
   workgroup_barrier();
   const uint32_t was = before;
   if (static_cast<int32_t>(was) <= keep) return;
   uint32_t end = pages_held(was, b);
   if (end > b.width) end = b.width;
-  const int32_t* table = b.tables + static_cast<uint64_t>(s) * b.width;
-  for (uint32_t j = pages_held(keep, b) + 4 * t; j < end; j += 4 * a.wg_size) {
-    const FourPages f = load_four(table, j, end);
+  while (j < end) {
     int32_t holders[4];
 #pragma unroll
     for (unsigned k = 0; k < 4; ++k)
-      holders[k] = f.page[k] < b.num_pages ? add_agent_i32(b.refs + f.page[k], -1) : 0;
+      holders[k] = j + k < end && f.page[k] < b.num_pages ? add_agent_i32(b.refs + f.page[k], -1) : 0;
     // pages that were handed out together often share a word
     uint32_t word = ~0u, bits = 0;
 #pragma unroll
@@ -636,6 +649,8 @@ MI355_DEVICE void page_free_body(const PageFreeArgs& a) {
       bits |= 1u << (f.page[k] % 32);
     }
     if (bits) or_agent_u32(b.bits + word, bits);
+    j += 4 * a.wg_size;
+    if (j < end) f = load_four(table, j, end);
   }
 }
 
