@@ -363,7 +363,7 @@ int mi355_blit_plan_rect_route(const mi355_pitched_ptr_t* dst, const mi355_dim3_
  * place, and a copy of the buffer is a copy of the whole state:
  *   head        word 0: the moves of the last compaction; the others are 0
  *   lengths     [max_seqs] tokens of each sequence, 0 for an empty one
- *   ref_counts  [num_pages] how many sequences hold a page
+ *   ref_counts  [num_pages] how many sequences hold a page; free pages are its zeros
  *   free_bits   bit q % 32 of word q / 32 is 1 where ref_counts[q] is 0
  *   tables      [max_seqs][max_pages_per_seq]; sequence s holds the pages
  *               tables[s][0 .. ceil(lengths[s] / rows)); entries from there on

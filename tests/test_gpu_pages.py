@@ -277,6 +277,41 @@ def test_copy_to_host_memory_and_back(torch_cuda, capi, engine):
             assert torch.equal(pool[:, held.long()], want)
 
 
+def test_copy_of_first_rows_to_host_memory_and_back(torch_cuda, capi, engine):
+    """Rows behind the valid ones stay as they are on either side, for pages of one run and
+    of several, in rows that are whole vectors and rows that are not."""
+    torch = torch_cuda
+    for runs, row_bytes in ((1, 2048), (6, 80), (3, 25)):
+        pages, rows, n = 120, 9, 100
+        dev = torch.randint(0, 256, (pages, runs, rows, row_bytes), dtype=torch.uint8, device="cuda:0")
+        host = torch.full((pages, runs, rows, row_bytes), 7, dtype=torch.uint8, pin_memory=True)
+        src = torch.randperm(pages, device="cuda:0", dtype=torch.int32)[:n].contiguous()
+        dst = torch.randperm(pages, device="cuda:0", dtype=torch.int32)[:n].contiguous()
+        valid = torch.randint(0, rows + 1, (n,), device="cuda:0", dtype=torch.int32)
+        torch.cuda.synchronize()
+        kept = (torch.arange(rows, device="cuda:0") < valid[:, None])[:, None, :, None]
+        spec = [(dev.data_ptr(), runs * rows * row_bytes, row_bytes, runs)]
+        with capi.Pages(engine, spec, pages, rows) as d, \
+                capi.Pages(engine, [(host.data_ptr(),) + spec[0][1:]], pages, rows) as h:
+            ok(capi, h.copy(dst.data_ptr(), src.data_ptr(), n, valid.data_ptr(), d, capi.ROUTE_DEVICE_TO_HOST))
+            ok(capi, engine.synchronize())
+            want = torch.full_like(dev, 7)
+            want[dst.long()] = torch.where(kept, dev[src.long()], want[dst.long()])
+            assert torch.equal(host, want.cpu())
+            before = dev.clone()
+            torch.cuda.synchronize()
+            ok(capi, d.copy(src.data_ptr(), dst.data_ptr(), n, valid.data_ptr(), h, capi.ROUTE_HOST_TO_DEVICE))
+            ok(capi, engine.synchronize())
+            assert torch.equal(dev, before)   # what went out came back, the rest was left
+            dev.zero_()
+            torch.cuda.synchronize()
+            ok(capi, d.copy(src.data_ptr(), dst.data_ptr(), n, valid.data_ptr(), h, capi.ROUTE_HOST_TO_DEVICE))
+            ok(capi, engine.synchronize())
+            back = torch.zeros_like(dev)
+            back[src.long()] = torch.where(kept, before[src.long()], back[src.long()])
+            assert torch.equal(dev, back)
+
+
 def test_pages_beyond_32_bits(torch_cuda, capi, engine):
     """Pages 3 GiB apart: the last one starts beyond 2^33."""
     torch = torch_cuda
