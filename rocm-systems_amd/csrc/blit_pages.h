@@ -39,7 +39,7 @@ struct __attribute__((aligned(64))) PagePlane {
   uint32_t run_bytes;     // rows * row_bytes; 0 where the page is one run
   uint32_t row_bytes;
   uint32_t runs;
-  uint64_t magic_run;     // magic_divisor(run_bytes)
+  uint32_t pad[2];
 };
 static_assert(sizeof(PagePlane) == 64, "one s_load_dwordx16");
 
@@ -288,7 +288,6 @@ inline uint32_t pages_planes(const mi355_blit_pages_desc_t& d, unsigned unroll, 
     r.magic_pieces = magic_divisor(r.pieces);
     r.first = first;
     r.run_bytes = p.runs > 1 ? d.rows * p.row_bytes : 0;
-    r.magic_run = magic_divisor(r.run_bytes);
     r.row_bytes = p.row_bytes;
     r.runs = p.runs;
     for (uint32_t k = 0; out && k < r.pieces; ++k) out[first + k] = r;
