@@ -430,8 +430,10 @@ int mi355_blit_pages_book(uint32_t num_pages, uint32_t max_seqs, uint32_t max_pa
  * and neither can mi355_blit_pages_destroy.  A missing plane or base, zero pages, rows,
  * runs or row_bytes, a pitch below the page's bytes, a book without sequences
  * or the other way round -> INVALID_ARGUMENT.  More than 4096 planes, a page of
- * more than 2^31-1 bytes in one plane, sequences of more than 2^31-1 tokens,
- * 2^32 pieces of 1 KiB or more in the pool, or more than the limits above -> OUT_OF_RESOURCES.
+ * more than 2^31-1 bytes in one plane or of more than 4 GiB in all of them,
+ * sequences of more than 2^31-1 tokens, 2^32 pieces of 1 KiB or more in the pool,
+ * or more than the limits above
+ * -> OUT_OF_RESOURCES.
  * The planes' and the book's memory stay the caller's and have to outlive the
  * object.  The object has to be destroyed before the handle: until then
  * mi355_blit_destroy answers INVALID_ARGUMENT and leaves the handle as it is. */

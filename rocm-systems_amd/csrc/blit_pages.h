@@ -186,6 +186,7 @@ constexpr uint32_t kMaxSeqs = MI355_BLIT_PAGES_MAX_SEQS;
 constexpr uint32_t kMaxPages = MI355_BLIT_PAGES_MAX_PAGES;
 static_assert(1024ull * (kMaxPages + 1) < 1ull << 32, "what 1024 sequences ask for is summed up in 32 bits");
 constexpr uint32_t kMaxPlanes = 4096;
+constexpr uint64_t kMaxPieces = 1u << 22;  // a page of 4 GiB over all planes
 // Every part of a book starts at a multiple of this many words.
 constexpr uint64_t kBookAlign = 64;
 
@@ -268,8 +269,8 @@ inline int pages_check(const mi355_blit_pages_desc_t* d, uint64_t* pieces) {
     if (end >> 64) return MI355_BLIT_ERROR_INVALID_ARGUMENT;
     total += (page + piece_bytes(1) - 1) / piece_bytes(1);
   }
-  // work items are counted in 32 bits
-  if (total * d->num_pages > 0xffffffffull) return MI355_BLIT_ERROR_OUT_OF_RESOURCES;
+  // work items are counted in 32 bits; the tables have a record for each piece
+  if (total > kMaxPieces || total * d->num_pages > 0xffffffffull) return MI355_BLIT_ERROR_OUT_OF_RESOURCES;
   *pieces = total;
   return MI355_BLIT_SUCCESS;
 }

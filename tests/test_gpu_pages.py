@@ -638,6 +638,7 @@ def test_refusals(torch_cuda, capi, engine, rand):
     assert status([(base, 1 << 63, 16, 1)]) == inv                 # beyond the address space
     assert status(good * 4097) == res
     assert status([(base, 1 << 40, 1 << 30, 2)], rows=1, pages=1) == res
+    assert status([(base, 1 << 40, 1 << 30, 1)] * 5, rows=1, pages=1) == res
     assert status(good, pages=capi.PAGES_MAX_PAGES + 1) == res
     assert status(good, seqs=capi.PAGES_MAX_SEQS + 1, width=2, where=book.data_ptr()) == res
     assert status(good, rows=4, seqs=2, width=1 << 29, where=book.data_ptr()) == res
