@@ -249,11 +249,13 @@ inline uint64_t plane_page_bytes(const mi355_blit_plane_t& p, uint32_t rows) {
 
 // What mi355_blit_pages_create takes; *pieces gets the number of the smallest pieces of a page.
 inline int pages_check(const mi355_blit_pages_desc_t* d, uint64_t* pieces) {
-  if (!d || !d->planes || d->n_planes == 0 || d->num_pages == 0 || d->rows == 0) return MI355_BLIT_ERROR_INVALID_ARGUMENT;
+  if (!d || !d->planes || d->n_planes == 0 || d->num_pages == 0 || d->rows == 0)
+    return MI355_BLIT_ERROR_INVALID_ARGUMENT;
   if ((d->max_seqs == 0) != (d->book == nullptr) || (d->max_seqs == 0) != (d->max_pages_per_seq == 0))
     return MI355_BLIT_ERROR_INVALID_ARGUMENT;
   if (reinterpret_cast<uintptr_t>(d->book) & 15) return MI355_BLIT_ERROR_INVALID_ARGUMENT;
-  if (d->n_planes > kMaxPlanes || d->num_pages > kMaxPages || d->max_seqs > kMaxSeqs) return MI355_BLIT_ERROR_OUT_OF_RESOURCES;
+  if (d->n_planes > kMaxPlanes || d->num_pages > kMaxPages || d->max_seqs > kMaxSeqs)
+    return MI355_BLIT_ERROR_OUT_OF_RESOURCES;
   // a sequence's tokens are counted in 31 bits
   if (static_cast<uint64_t>(d->max_pages_per_seq) * d->rows > 0x7fffffffull) return MI355_BLIT_ERROR_OUT_OF_RESOURCES;
   uint64_t total = 0;

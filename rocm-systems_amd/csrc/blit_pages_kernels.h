@@ -69,7 +69,10 @@ MI355_DEVICE void page_move_body(const PageMoveArgs& a, uint64_t first_wave) {
   const uint64_t total = static_cast<uint64_t>(n) * a.pieces;
   for (uint64_t w = first_wave; w < total; w += a.n_waves) {
     const uint32_t item = static_cast<uint32_t>(w);
+    // (the limits here and below hold, unless another call on the book has
+    // changed the count meanwhile; a branch for them costs 9 % of a compaction)
     uint32_t some_piece = div_magic(item, magic_n);
+    some_piece = some_piece < a.pieces ? some_piece : 0;
     uint32_t first = 0, pieces = a.even_pieces;
     uint64_t magic_pieces = a.magic_even;
     if (pieces) {
@@ -81,7 +84,8 @@ MI355_DEVICE void page_move_body(const PageMoveArgs& a, uint64_t first_wave) {
       first = p.first, pieces = p.pieces, magic_pieces = p.magic_pieces;
     }
     const uint32_t in_plane = item - n * first;
-    const uint32_t move = div_magic(in_plane, magic_pieces);
+    uint32_t move = div_magic(in_plane, magic_pieces);
+    move = move < n ? move : n - 1;
     const uint32_t offset = (in_plane - move * pieces) * piece_bytes(U);
     const uint32_t to = ld_uniform_u32(reinterpret_cast<const uint32_t*>(a.dst + move));
     const uint32_t from = ld_uniform_u32(reinterpret_cast<const uint32_t*>(a.src + move));
@@ -212,8 +216,11 @@ MI355_DEVICE uint32_t select_page(const BookPtrs& b, const uint32_t* groups, uin
 // The page with rank nth goes to the entry whose share of the running sum of
 // needs nth falls into.
 MI355_DEVICE void hand_out(const BookPtrs& b, uint32_t page, uint32_t nth, uint32_t start, uint32_t who, uint32_t slot) {
-  const uint64_t row = static_cast<uint64_t>(who & 0x7fffffffu) * b.width;
-  st_obj(b.tables + row + slot + (nth - start), static_cast<int32_t>(page));
+  const uint32_t seq = who & 0x7fffffffu;
+  const uint32_t at = slot + (nth - start);
+  // not so, unless another call on the book has changed the list meanwhile
+  if (seq >= b.max_seqs || at >= b.width) return;
+  st_obj(b.tables + static_cast<uint64_t>(seq) * b.width + at, static_cast<int32_t>(page));
   st_obj(b.refs + page, 1);
 }
 
@@ -469,7 +476,8 @@ MI355_DEVICE void page_assign_body(const PageFinishArgs& a) {
   const BookPtrs& b = a.book;
   const unsigned lane = thread_in_workgroup() & (kWave - 1);
   const uint32_t wanted = ld_uniform_u32(a.work.wanted);
-  for (uint32_t pair = static_cast<uint32_t>(global_wave(kMoveWaves)); pair < a.n_pairs; pair += a.assign_wgs * kMoveWaves) {
+  uint32_t pair = static_cast<uint32_t>(global_wave(kMoveWaves));
+  for (; pair < a.n_pairs; pair += a.assign_wgs * kMoveWaves) {
     if (wanted == 0) return;
     const uint32_t front = ld_uniform_u32(a.work.pairs + pair);
     if (front >= wanted) return;  // and so it is for every later pair
@@ -783,12 +791,20 @@ MI355_DEVICE void page_compact_plan_body(const PageCompactArgs& a) {
               select_page<true>(b, groups, a.lane_vecs, t));
 }
 
+// The moves that the first launch has counted; never more than there is room
+// for, whatever another call on the book may have left there.
+MI355_DEVICE uint32_t compact_moves(const PageCompactArgs& a) {
+  const uint32_t n = ld_uniform_u32(&a.moves.count->n);
+  return n < a.max_moves ? n : a.max_moves;
+}
+
 // The counts of the pages that move and where they go.
 MI355_DEVICE void page_compact_list_body(const PageCompactArgs& a) {
   const BookPtrs& b = a.book;
-  const uint32_t n = ld_uniform_u32(&a.moves.count->n);
+  const uint32_t n = compact_moves(a);
   const uint32_t live = ld_uniform_u32(a.live);
-  for (uint32_t pair = static_cast<uint32_t>(global_wave(kMoveWaves)); pair < a.n_pairs; pair += a.pair_wgs * kMoveWaves) {
+  uint32_t pair = static_cast<uint32_t>(global_wave(kMoveWaves));
+  for (; pair < a.n_pairs; pair += a.pair_wgs * kMoveWaves) {
     if (64 * pair >= live) return;
     const uint32_t front = ld_uniform_u32(a.pairs + pair);
     if (front >= n) return;  // the pages that move are all further down
@@ -853,14 +869,15 @@ template <bool NTL, int ST>
 MI355_DEVICE void page_compact_finish_body(const PageCompactFinishArgs& f) {
   const PageCompactArgs& a = f.compact;
   const uint32_t wg = workgroup_index();
-  const uint32_t n = ld_uniform_u32(&a.moves.count->n);
+  const uint32_t n = compact_moves(a);
   if (n == 0) return;
   if (wg < a.pair_wgs)
     page_compact_bits_body(a, n, static_cast<uint32_t>(global_wave(kMoveWaves)));
   else if (wg < a.pair_wgs + a.book.max_seqs)
     page_compact_tables_body(a, n, wg - a.pair_wgs);
   else
-    page_move_body<1, NTL, ST>(f.moves, global_wave(kMoveWaves) - static_cast<uint64_t>(kMoveWaves) * (a.pair_wgs + a.book.max_seqs));
+    page_move_body<1, NTL, ST>(f.moves, global_wave(kMoveWaves) -
+                                            static_cast<uint64_t>(kMoveWaves) * (a.pair_wgs + a.book.max_seqs));
 }
 
 // An empty book: no tokens, no holders, every page free, no table entry.
