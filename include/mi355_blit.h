@@ -182,7 +182,8 @@ typedef struct {
 int mi355_blit_create(int device_ordinal, mi355_blit_t** out);
 
 /* Replaces BlitKernel::Destroy (amd_blit_kernel.cpp:593-612).  Blocks until all
- * submitted commands have executed. */
+ * submitted commands have executed.  The handle is gone whatever it answers, but
+ * for INVALID_ARGUMENT where pools (mi355_blit_pages_create) still use it. */
 int mi355_blit_destroy(mi355_blit_t* h);
 
 /* Replaces the dispatch half of BlitKernel::SubmitLinearCopyCommand
@@ -439,7 +440,8 @@ int mi355_blit_pages_book(uint32_t num_pages, uint32_t max_seqs, uint32_t max_pa
 int mi355_blit_pages_create(mi355_blit_t* h, const mi355_blit_pages_desc_t* desc, mi355_blit_pages_t** out);
 
 /* Waits for the GPU, then frees the work memory.  Graphs that hold calls on the
- * object cannot be replayed any more. */
+ * object cannot be replayed any more.  Where it does not answer SUCCESS the object
+ * is still there. */
 int mi355_blit_pages_destroy(mi355_blit_pages_t* p);
 
 /* Empties the book: no tokens, every page free, -1 in every table entry.

@@ -214,7 +214,8 @@ class Blit:
     def close(self):
         if self.handle:
             st = self.lib.mi355_blit_destroy(self.handle)
-            self.handle = None
+            if st != ERROR_INVALID_ARGUMENT:  # which leaves it as it is: pools are open
+                self.handle = None
             check(st, "mi355_blit_destroy")
 
     def __enter__(self):
@@ -305,9 +306,8 @@ class Pages:
 
     def close(self):
         if self.handle:
-            st = self.lib.mi355_blit_pages_destroy(self.handle)
-            self.handle = None
-            check(st, "mi355_blit_pages_destroy")
+            check(self.lib.mi355_blit_pages_destroy(self.handle), "mi355_blit_pages_destroy")
+            self.handle = None  # (a refused one is still there)
 
     def __enter__(self):
         return self
