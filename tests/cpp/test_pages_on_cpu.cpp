@@ -12,6 +12,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <functional>
 #include <memory>
 #include <set>
 #include <string>
@@ -41,6 +42,9 @@ std::string g_at;
 void fail(const char* what) {
   if (g_failures++ < 20) std::printf("FAIL %s: %s\n", g_at.c_str(), what);
 }
+
+// What happens in front of every launch (nothing, usually).
+std::function<void()> g_meanwhile;
 
 struct Config {
   uint32_t pages, rows, seqs, width;
@@ -192,6 +196,7 @@ struct Cache {
 
   template <typename Args>
   static void run(void (*kernel)(Args), const Args& args, uint32_t grid, uint32_t wg) {
+    if (g_meanwhile) g_meanwhile();
     g_check.seal();
     g_reverse_grid = rnd() & 1 ? grid : 0;
     lane_emu::launch(kernel, args, grid, wg);
@@ -514,6 +519,37 @@ void random_words() {
   }
 }
 
+// Another call on the same book, which nobody has ordered with this one, may change the
+// work memory between two launches, or in the middle of one: any result, no access
+// outside.
+void work_memory_changes() {
+  Cache cache;
+  if (!cache.make(some_config(false))) return fail("a configuration was refused");
+  const Config& c = cache.pool.c;
+  const auto some_word = [&] {
+    return static_cast<uint32_t>(below(3) ? below(2 * c.pages + 2) : below(2) ? below(50) : rnd());
+  };
+  for (int turn = 0; turn < 4; ++turn) {
+    const uint32_t n = static_cast<uint32_t>(between(1, 40));
+    List x, y;
+    for (uint32_t i = 0; i < n; ++i)
+      x.push_back(static_cast<int32_t>(below(c.seqs))), y.push_back(static_cast<int32_t>(below(3 * c.rows)));
+    Words a(x), b(y), granted(List(n, 0)), out(List(c.pages + 2, 0));
+    cache.start(), cache.reads(a), cache.reads(b), cache.writes(granted), cache.writes(out);
+    g_meanwhile = [&] {
+      for (uint64_t i = 0; i < cache.work_words; ++i)
+        if (below(2)) cache.work[i] = some_word();
+      // a number of moves with the divisor of another
+      if (below(2)) *cache.moves.count = {static_cast<uint32_t>(between(1, 40)), 0, magic_divisor(some_word())};
+    };
+    cache.run_reserve(a, b, granted.p.get(), n);
+    cache.run_fork(a, b, granted.p.get(), n);
+    if (c.pages / 2) cache.run_compact(c.pages / 2, out.p.get());
+    g_meanwhile = nullptr;
+    ++g_calls;
+  }
+}
+
 // More pages than one vector of free bits for each lane covers, and more than one
 // round of entries that ask for them.
 void large_pool() {
@@ -555,11 +591,12 @@ int main(int argc, char** argv) {
   unsigned shard = 0, shards = 1;
   for (int i = 1; i < argc; ++i)
     if (!std::strcmp(argv[i], "--shard") && i + 1 < argc && std::sscanf(argv[++i], "%u/%u", &shard, &shards) != 2) return 2;
-  for (unsigned k = shard; k < 240; k += shards) {
+  for (unsigned k = shard; k < 300; k += shards) {
     g_state = 0x9E3779B97F4A7C15ull * (k + 1);
     g_at = "case " + std::to_string(k);
     if (k == 0) large_pool();
     else if (k == 1) long_sequences();
+    else if (k >= 240) work_memory_changes();
     else if (k % 12 == 1) random_life(4, true);
     else if (k % 4 == 2) random_copies();
     else if (k % 4 == 3) random_words();
