@@ -1115,8 +1115,7 @@ int mi355_blit_pages_free(mi355_blit_pages_t* p, const int32_t* seqs, const int3
 
 int mi355_blit_pages_compact(mi355_blit_pages_t* p, uint32_t max_moves, int32_t* moves, void* stream) {
   if (!p || !p->has_book || !aligned_list(moves)) return MI355_BLIT_ERROR_INVALID_ARGUMENT;
-  // a hole for each page that moves
-  const uint32_t most = max_moves < p->num_pages / 2 ? max_moves : p->num_pages / 2;
+  const uint32_t most = most_page_moves(max_moves, p->num_pages);
   if (most == 0) return MI355_BLIT_SUCCESS;
   std::lock_guard<std::mutex> g(p->h->lock);
   DeviceScope scope(p->h->device);

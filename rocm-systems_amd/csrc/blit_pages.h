@@ -319,6 +319,13 @@ static_assert(64ull * kMaxList * 1024 <= kMaxGridWorkItems, "work-items of a gri
 // page's bit, 10.8 so; 128 sequences 12.3 and 11.1; 100 in tables of 700 8.5 and 11.5.
 constexpr uint64_t kFreeByCounts = 1u << 17;
 
+// Moves that a compaction may make: each takes a page that is in use and a free
+// one.  (One page: none, but the launches say so in the book's head.)
+inline uint32_t most_page_moves(uint32_t max_moves, uint32_t num_pages) {
+  const uint32_t pairs = num_pages > 1 ? num_pages / 2 : 1;
+  return max_moves < pairs ? max_moves : pairs;
+}
+
 // Moves of a compaction that its first launch finds by itself.
 constexpr uint32_t kListedAtOnce = 1024;
 

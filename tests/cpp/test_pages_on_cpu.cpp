@@ -569,6 +569,27 @@ void large_pool() {
   cache.reserve(gone, List(gone.size(), 300));  // does not fit to its end
 }
 
+// A pool of one page has nowhere to move it: no moves, and the head says so.
+void one_page() {
+  Config c;
+  c.rows = 4, c.seqs = 2, c.width = 1, c.pages = 1;
+  c.planes.push_back({nullptr, 0, 24, 1});
+  Cache cache;
+  if (!cache.make(c)) return fail("a configuration was refused");
+  for (int turn = 0; turn < 2; ++turn) {
+    cache.book[0] = 7;
+    Words out(List(2, -5));
+    cache.start(), cache.writes(out);
+    cache.run_compact(most_page_moves(9, c.pages), out.p.get());
+    cache.check("compact of one page");
+    if (out.p[0] != -5) fail("compact of one page: moves");
+    cache.reserve({1}, {3});
+  }
+  if (most_page_moves(9, 1) != 1 || most_page_moves(9, 2) != 1 || most_page_moves(9, 7) != 3 ||
+      most_page_moves(9, 100) != 9 || most_page_moves(0, 1) != 0 || most_page_moves(0, 100) != 0)
+    fail("room for moves");
+}
+
 // Tables of several stretches of kTableChunk pages.
 void long_sequences() {
   Config c;
@@ -591,11 +612,12 @@ int main(int argc, char** argv) {
   unsigned shard = 0, shards = 1;
   for (int i = 1; i < argc; ++i)
     if (!std::strcmp(argv[i], "--shard") && i + 1 < argc && std::sscanf(argv[++i], "%u/%u", &shard, &shards) != 2) return 2;
-  for (unsigned k = shard; k < 300; k += shards) {
+  for (unsigned k = shard; k < 301; k += shards) {
     g_state = 0x9E3779B97F4A7C15ull * (k + 1);
     g_at = "case " + std::to_string(k);
     if (k == 0) large_pool();
     else if (k == 1) long_sequences();
+    else if (k == 300) one_page();
     else if (k >= 240) work_memory_changes();
     else if (k % 12 == 1) random_life(4, true);
     else if (k % 4 == 2) random_copies();
