@@ -569,6 +569,31 @@ void large_pool() {
   cache.reserve(gone, List(gone.size(), 300));  // does not fit to its end
 }
 
+// The rule that picks a kernel, on both sides of each of its limits; for first
+// rows half of the pages' bytes count.
+void launch_rule() {
+  const uint32_t pieces[2] = {1024, 256};
+  const uint64_t page = 1 << 20;
+  const uint32_t streams = kMoveStreams / page, nt = kMoveNtStores / page;
+  for (unsigned cut = 0; cut < 2; ++cut)
+    for (uint32_t route = 0; route < 3; ++route)
+      for (uint32_t pages : {1u, streams - 1, streams, nt - 1, nt, 4 * nt}) {
+        const uint64_t n = static_cast<uint64_t>(pages) * (cut ? 2 : 1);
+        const PageMovePlan p = plan_page_moves(n, 0, cut, pieces, page, 256, route, 128);
+        const uint32_t store = route == MI355_BLIT_ROUTE_DEVICE_TO_HOST ? MI355_BLIT_STORE_SYSTEM_WT
+                               : pages >= nt                            ? MI355_BLIT_STORE_NT
+                               : pages >= streams                       ? MI355_BLIT_STORE_AGENT_WT
+                                                                        : MI355_BLIT_STORE_CACHED;
+        if (p.table != cut || p.nt_load != (pages >= streams) || p.store_policy != store) fail("rule of kernels");
+        const uint64_t want = n * pieces[cut] / kMoveWaves;
+        if (p.grid != (route ? (want < 128 ? want : 128) : want)) fail("rule of grids");
+      }
+  // a list of unknown length: its room, up to so many workgroups for each CU
+  if (plan_page_moves(500, kMostListed, false, pieces, page, 256, 0, 128).grid != 500 * 256 ||
+      plan_page_moves(513, kMostListed, false, pieces, page, 256, 0, 128).grid != kMostListed * 256)
+    fail("rule of grids for lists");
+}
+
 // A pool of one page has nowhere to move it: no moves, and the head says so.
 void one_page() {
   Config c;
@@ -612,12 +637,13 @@ int main(int argc, char** argv) {
   unsigned shard = 0, shards = 1;
   for (int i = 1; i < argc; ++i)
     if (!std::strcmp(argv[i], "--shard") && i + 1 < argc && std::sscanf(argv[++i], "%u/%u", &shard, &shards) != 2) return 2;
-  for (unsigned k = shard; k < 301; k += shards) {
+  for (unsigned k = shard; k < 302; k += shards) {
     g_state = 0x9E3779B97F4A7C15ull * (k + 1);
     g_at = "case " + std::to_string(k);
     if (k == 0) large_pool();
     else if (k == 1) long_sequences();
     else if (k == 300) one_page();
+    else if (k == 301) launch_rule();
     else if (k >= 240) work_memory_changes();
     else if (k % 12 == 1) random_life(4, true);
     else if (k % 4 == 2) random_copies();
