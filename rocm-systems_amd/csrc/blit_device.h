@@ -217,9 +217,6 @@ MI355_DEVICE int32_t min_agent_i32(int32_t* p, int32_t v) {
 MI355_DEVICE uint32_t or_agent_u32(uint32_t* p, uint32_t v) {
   return __hip_atomic_fetch_or(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-MI355_DEVICE uint32_t and_agent_u32(uint32_t* p, uint32_t v) {
-  return __hip_atomic_fetch_and(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
 // Returns when the wave's loads, stores and atomics have been performed.
 MI355_DEVICE void wait_for_memory() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 

@@ -37,9 +37,6 @@ MI355_DEVICE int32_t min_agent_i32(int32_t* p, int32_t v) {
 MI355_DEVICE uint32_t or_agent_u32(uint32_t* p, uint32_t v) {
   return checked_change(p, [v](uint32_t w) { return w | v; });
 }
-MI355_DEVICE uint32_t and_agent_u32(uint32_t* p, uint32_t v) {
-  return checked_change(p, [v](uint32_t w) { return w & v; });
-}
 MI355_DEVICE void wait_for_memory() {}
 
 // LDS is ordinary memory here (AddressSanitizer watches it)
