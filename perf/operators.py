@@ -361,12 +361,20 @@ def _bits_of(pool):
     return pool if pool.dtype == torch.uint8 else pool.view(torch.int16)
 
 
+def _stream():
+    """The stream that torch's work is on, so that the calls come behind what made their inputs and in
+    front of what reads their outputs.  torch names its default stream 0, which the calls take
+    for the handle's own; HIP's name for it is hipStreamLegacy, 1."""
+    return torch.cuda.current_stream().cuda_stream or 1
+
+
 def run(st):
     op = st["op"]
+    stream = _stream() if own else None
     if op == "copy":
         if own:
             valid = st["valid"].data_ptr() if st["valid"] is not None else None
-            _ok(st["to"].copy(st["dst"].data_ptr(), st["src"].data_ptr(), st["n"], valid=valid, src=st["from"]))
+            _ok(st["to"].copy(st["dst"].data_ptr(), st["src"].data_ptr(), st["n"], valid=valid, src=st["from"], stream=stream))
         else:
             _move(st["other"], st["dst"].long(), st["pool"], st["src"].long(), st["valid"], st["rows"])
         return {"pool": _bits_of(st["other"])}
@@ -374,15 +382,15 @@ def run(st):
     if own:
         blit = _engine["blit"]
         pages = st["pages_of"]
-        _ok(blit.copy(b.buf.data_ptr(), st["snapshot"].data_ptr(), 4 * b.buf.numel()))
+        _ok(blit.copy(b.buf.data_ptr(), st["snapshot"].data_ptr(), 4 * b.buf.numel(), stream=stream))
         if op == "reserve":
-            _ok(pages.reserve(st["list"].data_ptr(), st["add"].data_ptr(), st["n"], granted=st["granted"].data_ptr()))
+            _ok(pages.reserve(st["list"].data_ptr(), st["add"].data_ptr(), st["n"], granted=st["granted"].data_ptr(), stream=stream))
         elif op == "fork":
-            _ok(pages.fork(st["list"].data_ptr(), st["children"].data_ptr(), st["n"], granted=st["granted"].data_ptr()))
+            _ok(pages.fork(st["list"].data_ptr(), st["children"].data_ptr(), st["n"], granted=st["granted"].data_ptr(), stream=stream))
         elif op == "free":
-            _ok(pages.free(st["list"].data_ptr(), st["n"], keep=st["keep"].data_ptr() if st["keep"] is not None else None))
+            _ok(pages.free(st["list"].data_ptr(), st["n"], keep=st["keep"].data_ptr() if st["keep"] is not None else None, stream=stream))
         else:
-            _ok(pages.compact(st["budget"]))
+            _ok(pages.compact(st["budget"], stream=stream))
     else:
         b.buf.copy_(st["snapshot"])
         {"reserve": _plain_reserve, "fork": _plain_fork, "free": _plain_free, "compact": _plain_compact}[op](st, b)
