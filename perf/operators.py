@@ -27,6 +27,7 @@ The operators that change a book start every pass from the same book: a pass beg
 copying a snapshot over it, as a program does that runs a step speculatively.
 """
 import math
+import weakref
 
 import numpy as np
 import torch
@@ -198,10 +199,14 @@ def _own_pages(case, pool, book=None):
     pitch = pool.stride(1) * pool.element_size()
     planes = [(pool[p].data_ptr(), pitch, case["row_bytes"], case["runs"]) for p in range(case["planes"])]
     if book is None:
-        return capi.Pages(blit, planes, case["pages"], case["rows"])
-    where = capi.book_layout(case["pages"], case["seqs"], case["width"])
-    assert (where.lengths, where.ref_counts, where.free_bits, where.tables, where.words) == _layout(case)
-    return capi.Pages(blit, planes, case["pages"], case["rows"], case["seqs"], case["width"], book.buf.data_ptr())
+        pages = capi.Pages(blit, planes, case["pages"], case["rows"])
+    else:
+        where = capi.book_layout(case["pages"], case["seqs"], case["width"])
+        assert (where.lengths, where.ref_counts, where.free_bits, where.tables, where.words) == _layout(case)
+        pages = capi.Pages(blit, planes, case["pages"], case["rows"], case["seqs"], case["width"], book.buf.data_ptr())
+    # closed with the state that holds it; at the end of the process it goes with the process
+    weakref.finalize(pages, pages.lib.mi355_blit_pages_destroy, pages.handle).atexit = False
+    return pages
 
 
 def prepare(case, seed):
