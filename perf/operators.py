@@ -369,8 +369,10 @@ def _bits_of(pool):
 def _stream():
     """The stream that torch's work is on, so that the calls come behind what made their inputs and in
     front of what reads their outputs.  torch names its default stream 0, which the calls take
-    for the handle's own; HIP's name for it is hipStreamLegacy, 1."""
-    return torch.cuda.current_stream().cuda_stream or 1
+    for the handle's own; HIP's name for it is hipStreamLegacy, 1.  (torch.cuda.current_stream() makes a
+    Python object for it, 2.7 us, as long as a call; this is the number alone, as code that torch
+    generates asks for it.)"""
+    return torch._C._cuda_getCurrentRawStream(0) or 1
 
 
 def run(st):
