@@ -385,7 +385,8 @@ int mi355_blit_plan_rect_route(const mi355_pitched_ptr_t* dst, const mi355_dim3_
  * or in graphs that are replayed at the same time, without an ordering between
  * them -- race and are the caller's to order.  Copies use none, and race only
  * with what writes the pages that they name.  stream is a hipStream_t, or NULL
- * for the handle's own (which is not ordered with the default stream).  Like the
+ * for the handle's own, which is not ordered with any other; the default stream
+ * (torch's, unless another is set) is hipStreamLegacy here, not NULL.  Like the
  * allocation-free batch these commands are not entered in the pending-bytes
  * ledger, and neither mi355_blit_set_tuning nor mi355_blit_last_launch_info
  * knows of them. */

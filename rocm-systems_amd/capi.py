@@ -292,8 +292,9 @@ class Pages:
     """Owner of one mi355_blit_pages_t: the pages of a key/value cache, with a
     book (max_seqs, max_pages_per_seq and the device address of its buffer) or, for
     copies only, without.  planes: (base, pitch, row_bytes, runs) of each.  Methods
-    map 1:1 to the C ABI; lists are device addresses of int32.  Close it before the
-    Blit it was made with."""
+    map 1:1 to the C ABI; lists are device addresses of int32.  stream: None is the
+    Blit's own, 1 (hipStreamLegacy) the default stream, whose cuda_stream in torch is 0.
+    Close it before the Blit it was made with."""
 
     def __init__(self, blit, planes, num_pages, rows, max_seqs=0, max_pages_per_seq=0, book=None):
         self.lib = load()
