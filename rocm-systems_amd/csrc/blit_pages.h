@@ -19,9 +19,11 @@ namespace mi355 {
 
 // A wave moves a piece of a page at a time: 16 bytes for each lane, or four
 // times that where the first rows of the pages are moved only, so that fewer
-// waves find nothing to do (190 pages of 24 planes, half of their rows: 13.3 us
-// against 15.8; 600 pages of 1 MiB, half of their rows: 134 against 153; whole
-// pages, 800 of 1 MiB: 285 us with 1 KiB, 330 with 4 KiB).
+// waves go through the longer chain of loads in front of such a move, and fewer find
+// nothing to do (4 KiB against 1 KiB: 190 pages of 24 planes, half of their 33 rows
+// of 80 bytes in 5 runs, 13.5 us against 19.5; 600 pages of 1 MiB, half of their
+// rows, 137 against 482; whole pages, 800 of 1 MiB: 285 us with 1 KiB, 330 with
+// 4 KiB).
 constexpr unsigned kPieceUnrolls[] = {1, 4};
 constexpr uint32_t piece_bytes(unsigned unroll) { return kWave * 16 * unroll; }
 

@@ -21,6 +21,9 @@ namespace mi355 {
 // MiB, and not in all of them (512 pages of 64 planes of 32 KiB, 1 GiB each way: 369 us,
 // 5.8 TB/s, against 403 us in the order move, plane, piece; a linear copy of as many bytes 313).
 // Bound by memory: the counters show as many bytes read and written as the pages have.
+// First rows are bound by latency instead (below, and 600 pages of 1 MiB, half of
+// their rows, 629 MB: 137 us, 4.6 TB/s): a lane's four vectors each have a
+// condition of their own, and the compiler waits for each before the next.
 // ---------------------------------------------------------------------------
 
 // A page of several runs of which only the first rows are moved, `limit` bytes
@@ -31,7 +34,12 @@ namespace mi355 {
 // take at least as many units each as their piece has, the last ones none.  246
 // pages of 12 planes, half of their 32 rows of 42 bytes in 7 runs: 7.5 us, and 24.5
 // where vectors that lie across an end go byte by byte; 190 pages of 24
-// planes in runs of 33 rows of 80 bytes 14.6, and 15.5 over all vectors of the page.
+// planes in 5 runs of 33 rows of 80 bytes 14.6, and 15.5 over all vectors of the page.
+// Bound by latency: the waves of the latter spend three quarters of their time
+// waiting, behind the loads that lead to their rows and then for up to four vectors a lane
+// one after the other, and half of them find nothing to do; 34.8 MB are read and 32.9
+// written for 31.8.  (As many bytes of whole pages take 13.4 us, a linear copy 9.3; a variant
+// with four vectors a lane on the way at once was slower, 17.1.)
 template <int U, bool NTL, int ST>
 MI355_DEVICE void move_cut_runs(uint8_t* dp, const uint8_t* sp, const PagePlane& g, unsigned piece, unsigned pieces,
                                 unsigned limit, unsigned lane) {
@@ -281,7 +289,11 @@ MI355_DEVICE ReserveEntry load_reserve_entry(const PageReserveArgs& a, uint32_t 
 // its count, free bits) and a dozen barriers.  48 sequences that get a token each
 // 5.6 us and 2 for the second launch; 300 prompts, 19,000 pages 7.1 and 4.9 (one
 // workgroup that hands out all of them itself 244); 256 forks of 32 prompts of which 224
-// copy their last page 9.0, and 18.3 for 115 MB of copies (6.3 TB/s).
+// copy their last page 9.0, and 18.3 for 115 MB of copies (6.3 TB/s).  In pools of
+// more than 131,072 pages a lane goes through its stretch of the free bits one vector
+// after the other: for 48 sequences that get a page each the first launch takes 7.0 us
+// with 4,096 and with 131,072 pages, 22 with 2,000,000, 47 with 4,194,240.  8,192
+// entries take 58 us, 1024 at a time.
 MI355_DEVICE void page_reserve_body(const PageReserveArgs& a) {
   MI355_LDS uint32_t scan_a[16], scan_b[16];
   MI355_LDS uint32_t keys[kSlots], first[kSlots], asked[kSlots];
@@ -531,10 +543,11 @@ MI355_DEVICE FourPages load_four(const int32_t* table, uint32_t j, uint32_t end)
 // another may already have written: a child that an earlier entry names too is
 // left alone, and so is one whose parent is named as a child.
 //
-// The atomic additions are what takes time (the device does 20 of them in a
-// nanosecond, whatever their addresses), so the first entry that names a parent
-// adds to its pages' counts for all that do; an entry that is refused for its
-// child's sake, which the others cannot see, takes its own share off again.
+// The atomic additions are what takes time (at addresses that differ the device does
+// some 20 of them in a nanosecond, those to one cache line follow each other 2 to 5 ns
+// apart), so the first entry that names a parent adds to its pages' counts for all
+// that do; an entry that is refused for its child's sake, which the others cannot
+// see, takes its own share off again.
 // 1000 children of 90 parents, 560 pages each: 7.6 us, and 27.5 with an addition
 // for each child and page; 64 children of 16 parents 3.8.
 //
@@ -663,14 +676,16 @@ MI355_DEVICE void page_free_body(const PageFreeArgs& a) {
   }
 }
 
-// The same for many pages, in two launches.  The device does some 20 atomics in
-// a nanosecond, so there is one for each page, whose result nobody waits for, and
+// The same for many pages, in two launches.  The device does some 20 atomics in a
+// nanosecond, so there is one for each page, whose result nobody waits for, and
 // the second launch makes the free bits from the counts and shortens the
 // sequences (306,000 pages of 850 sequences: 28 us with the free bits by atomics,
 // 17 so; the tails of 850 sequences that share their pages, 150,000 pages in all,
-// 9.5 and 2.3 us).  A workgroup for each entry and a.chunk pages of its table; the
-// first entry that names a sequence acts for all that do, with the smallest keep
-// of theirs.
+// 9.5 and 2.3 us).  Where many hold the same few pages the counts are in a few cache
+// lines, and the additions follow each other: 1000 sequences of one prefix of 300
+// pages 78 us, of 300 pages each 6.1; 8192 sequences of one prefix of 10 pages 378.  A
+// workgroup for each entry and a.chunk pages of its table; the first entry that
+// names a sequence acts for all that do, with the smallest keep of theirs.
 MI355_DEVICE void page_free_counts_body(const PageFreeArgs& a) {
   MI355_LDS uint32_t again, least;
   const BookPtrs& b = a.book;
@@ -740,7 +755,8 @@ MI355_DEVICE void page_free_finish_body(const PageFreeArgs& a) {
 // the free bits and how many pages move, and one between the two, over the
 // whole device, finds for each hole the page that comes to it.  Bound by memory
 // where much moves (3,500 pages of 1 MiB of which 815 move: 4.6, 4.7 and 274 us,
-// 6.2 TB/s), by the launches otherwise (24 of 3,000 pages: 4.8 and 5.0 us).
+// 6.2 TB/s), by the launches otherwise (24 of 3,000 pages: 4.8 and 5.0 us; the first
+// launch in a pool of 2,000,000 pages 49).
 
 // Move k, of page `from` to page `to`: the list, the counts, and what the caller wants to know.
 MI355_DEVICE void list_move(const PageCompactArgs& a, uint32_t k, uint32_t from, uint32_t to) {
@@ -838,7 +854,8 @@ MI355_DEVICE void page_compact_list_body(const PageCompactArgs& a) {
   }
 }
 
-// The tables, a workgroup of 256 lanes for each sequence.  The pages that moved
+// The tables, a workgroup of 256 lanes for each sequence, whatever its length: 200
+// sequences of 500 pages 3.2 us, one of 98,000 109.  The pages that moved
 // are the highest ones, so every held page from the lowest of them on has moved.
 MI355_DEVICE void page_compact_tables_body(const PageCompactArgs& a, uint32_t n, uint32_t s) {
   const BookPtrs& b = a.book;
