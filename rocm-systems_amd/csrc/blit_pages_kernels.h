@@ -544,7 +544,7 @@ MI355_DEVICE FourPages load_four(const int32_t* table, uint32_t j, uint32_t end)
 // left alone, and so is one whose parent is named as a child.
 //
 // The atomic additions are what takes time (at addresses that differ the device does
-// some 20 of them in a nanosecond, those to one cache line follow each other 2 to 5 ns
+// up to 50 of them in a nanosecond, those to one cache line follow each other 2 to 5 ns
 // apart), so the first entry that names a parent adds to its pages' counts for all
 // that do; an entry that is refused for its child's sake, which the others cannot
 // see, takes its own share off again.
@@ -676,8 +676,8 @@ MI355_DEVICE void page_free_body(const PageFreeArgs& a) {
   }
 }
 
-// The same for many pages, in two launches.  The device does some 20 atomics in a
-// nanosecond, so there is one for each page, whose result nobody waits for, and
+// The same for many pages, in two launches.  Atomics are what takes time (see the
+// fork), so there is one for each page, whose result nobody waits for, and
 // the second launch makes the free bits from the counts and shortens the
 // sequences (306,000 pages of 850 sequences: 28 us with the free bits by atomics,
 // 17 so; the tails of 850 sequences that share their pages, 150,000 pages in all,
